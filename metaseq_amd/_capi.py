@@ -243,6 +243,25 @@ HYBRID_SIGNATURES = {
 HYBRID_OTHER_SYMBOLS = ["msa_hybrid_destroy", "msa_hybrid_workspace_bytes",
                         "msa_delta_scratch_floats"]
 
+# ---- the paged cache, in libmetaseq_amd.so (include/metaseq_paged.h) ------------------------
+MSA_F16 = 2
+MSA_PAGES_SAME, MSA_PAGES_E4M3, MSA_PAGES_INT8 = 0, 1, 2
+PagedCacheC = _struct("PagedCacheC", "msa_paged_cache", (c_int, "dtype format kv_heads hd page pages"),
+                      (c_void_p, "k_pages v_pages k_exp v_exp"))
+PagedBatchC = _struct("PagedBatchC", "msa_paged_batch", (c_int, "M nseq max_count key_bound blocks"),
+                      (c_int64, "table_stride"), (c_void_p, "seq_start seq_pos table"))
+PagedAttentionArgs = _struct(
+    "PagedAttentionArgs", "msa_paged_attention_args", (c_int, "heads"), (c_void_p, "q"), (c_int64, "ldq"),
+    (c_void_p, "out"), (c_int64, "ldo"), (c_int, "out_mb window sinks"), (c_float, "scale"),
+    (c_void_p, "workspace"), (c_int64, "workspace_bytes"))
+_PC, _PB, _PA = (ctypes.POINTER(s) for s in (PagedCacheC, PagedBatchC, PagedAttentionArgs))
+PAGED_SIGNATURES = {
+    "msa_paged_append": [_PC, _PB, _P, c_int64, _P, c_int64, _P],
+    "msa_paged_read": [_PC, _PB, _P, c_int64, _P, c_int64, _P],
+    "msa_paged_attention_workspace_bytes": [_PC, _PB, _PA],
+    "msa_paged_attention": [_PC, _PB, _PA, _P],
+}
+
 _lib = None
 _hybrid_lib = None
 
@@ -285,10 +304,11 @@ def load():
     if _lib is not None:
         return _lib
     lib = _open(LIB_PATH)
-    for name, args in SIGNATURES.items():
+    for name, args in list(SIGNATURES.items()) + list(PAGED_SIGNATURES.items()):
         fn = getattr(lib, name)
         fn.argtypes = args
         fn.restype = c_int
+    lib.msa_paged_attention_workspace_bytes.restype = c_int64
     lib.msa_lm_head_select_workspace_bytes.argtypes = [c_int]
     lib.msa_lm_head_select_workspace_bytes.restype = c_int64
     lib.msa_decoder_destroy.argtypes = [_P]

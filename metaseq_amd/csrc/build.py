@@ -17,13 +17,16 @@ LIBS = {"core": os.path.join(HERE, "libmetaseq_amd.so"),
 LIB = LIBS["core"]
 SOURCES = {
     "core": ["capi.hip", "layernorm.hip", "embed.hip", "gemm.hip", "gemm_queue_f16.hip", "gemm_queue_i8.hip", "attention.hip",
-             "attention_prefill.hip", "sampling.hip", "probe.hip", "decoder_step.hip"],
+             "attention_prefill.hip", "paged_cache.hip", "paged_attention.hip", "paged_attention_f16.hip",
+             "paged_attention_bf16.hip", "paged_attention_e4m3.hip", "paged_attention_i8.hip", "sampling.hip", "probe.hip",
+             "decoder_step.hip"],
     "hybrid": ["capi.hip", "gemm_bf16.hip", "gemm_bf16_post.hip", "gemm_queue_bf16.hip", "group_linear.hip", "moe.hip",
                "rmsnorm.hip", "recurrent.hip", "delta_chunks.hip", "latent_attention.hip",
                "grouped_attention.hip", "hybrid_step.hip"],
 }
-HEADERS = ["common.h", "gemm_kernels.h", "gemm_queue.h", "attention_tiles.h",
+HEADERS = ["common.h", "gemm_kernels.h", "gemm_queue.h", "attention_tiles.h", "paged.h", "paged_attention.h",
            os.path.join("..", "..", "include", "metaseq_amd.h"),
+           os.path.join("..", "..", "include", "metaseq_paged.h"),
            os.path.join("..", "..", "include", "metaseq_hybrid.h")]
 # (the last flag: a kernel's first fourteen argument words are in registers when a wave starts, where it would read them
 # from memory first, some 0.3 us in front of its first load)
@@ -39,7 +42,11 @@ FLAGS = [
 # and copies each one out)
 EXTRA_FLAGS = {"attention_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
                "latent_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
-               "grouped_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+               "grouped_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+               "paged_attention_f16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+               "paged_attention_bf16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+               "paged_attention_e4m3.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+               "paged_attention_i8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def _hipcc():

@@ -1,0 +1,124 @@
+// Attention over pages: which kernel takes a batch, how keys are split, and the sum of the splits.
+#include "paged_attention.h"
+
+void msa_launch_paged_rows_f16(const PagedAttention& a, int hd, int row_tiles, hipStream_t stream);
+void msa_launch_paged_rows_bf16(const PagedAttention& a, int hd, int row_tiles, hipStream_t stream);
+void msa_launch_paged_rows_e4m3(const PagedAttention& a, int hd, int row_tiles, hipStream_t stream);
+void msa_launch_paged_rows_i8(const PagedAttention& a, int hd, int row_tiles, hipStream_t stream);
+
+namespace {
+
+// One wave per (row, query head): out = sum of the splits' sums, each relative to its own maximum.
+__global__ __launch_bounds__(64) void paged_combine_kernel(PagedAttention a, int hd) {
+  const int lane = threadIdx.x, r = blockIdx.x, head = blockIdx.y;
+  const int s = __builtin_amdgcn_readfirstlane(paged_sequence_of(a.seq_start, a.nseq, r));
+  if (s >= a.nseq || r >= a.seq_start[a.nseq] || a.seq_pos[s] < 0 || a.seq_start[s] < 0 || r - a.seq_start[s] >= a.max_count) return;
+  const float* part = a.partial + ((int64_t)r * a.heads + head) * a.splits * (hd + 4);
+  float top = -INFINITY;
+  for (int i = lane; i < a.splits; i += 64) top = fmaxf(top, part[(int64_t)i * (hd + 4) + hd]);
+  top = wave_max(top);
+  const float off = top == -INFINITY ? 0.f : top;
+  float o[4] = {0.f, 0.f, 0.f, 0.f}, total = 0.f;
+  for (int i = 0; i < a.splits; ++i) {
+    const float* p = part + (int64_t)i * (hd + 4);
+    const float w = __builtin_amdgcn_exp2f(p[hd] - off);
+    total += w * p[hd + 1];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (lane * 4 < hd) o[k] += w * p[lane * 4 + k];
+  }
+  if (lane * 4 >= hd) return;
+  const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
+  uint16_t w[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    w[k] = a.bf16 ? __builtin_bit_cast(uint16_t, (bf16_t)(o[k] * inv)) : __builtin_bit_cast(uint16_t, (half_t)(o[k] * inv));
+  const int d = head * hd + lane * 4;
+  const int64_t at = a.out_mb > 0 ? packed_act_offset(r, d, a.out_mb) : (int64_t)r * a.ldo + d;
+  *(pg_u2*)((uint16_t*)a.out + at) = pg_u2{(uint32_t)w[0] | (uint32_t)w[1] << 16, (uint32_t)w[2] | (uint32_t)w[3] << 16};
+}
+
+struct Plan {
+  int row_tiles, row_blocks, splits;
+};
+
+Plan plan_of(const msa_paged_cache& c, const msa_paged_batch& b, const msa_paged_attention_args& a) {
+  Plan p;
+  const int64_t rows = (int64_t)b.max_count * (a.heads / c.kv_heads);
+  p.row_tiles = rows <= 16 ? 1 : 2;
+  p.row_blocks = (int)((rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
+  // keys that a row block can see, in tiles of the format; a split is at least one tile per wave
+  int64_t keys = b.key_bound;
+  if (a.window > 0) keys = keys < (int64_t)a.window + a.sinks + b.max_count ? keys : (int64_t)a.window + a.sinks + b.max_count;
+  const int kt = c.format == MSA_PAGES_SAME ? 32 : 64;
+  const int64_t tiles = (keys + kt - 1) / kt, groups = (int64_t)b.nseq * p.row_blocks * c.kv_heads;
+  const int64_t most = (tiles + PA_NW - 1) / PA_NW;
+  int64_t s = groups >= 512 ? 1 : 1024 / groups;
+  if (s > most) s = most;
+  if (s > 128) s = 128;
+  p.splits = s < 1 ? 1 : (int)s;
+  return p;
+}
+
+int check(const msa_paged_cache* c, const msa_paged_batch* b, const msa_paged_attention_args* a) {
+  const int rc = msa_paged_check(c, b, "msa_paged_attention");
+  if (rc) return rc;
+  MSA_REQUIRE(a, MSA_ERR_INVALID_ARG, "msa_paged_attention: null pointer");
+  MSA_REQUIRE(a->heads >= 1 && a->heads % c->kv_heads == 0, MSA_ERR_INVALID_ARG,
+              "msa_paged_attention: %d query heads are no multiple of %d key/value heads", a->heads, c->kv_heads);
+  MSA_REQUIRE(a->heads <= 65535, MSA_ERR_INVALID_ARG, "msa_paged_attention: at most 65535 heads");
+  MSA_REQUIRE(a->window >= 0 && a->sinks >= 0, MSA_ERR_INVALID_ARG, "msa_paged_attention: window and sinks must not be negative");
+  MSA_REQUIRE(a->scale > 0.f && a->scale < INFINITY, MSA_ERR_INVALID_ARG, "msa_paged_attention: scale must be positive and finite");
+  return MSA_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t msa_paged_attention_workspace_bytes(const msa_paged_cache* c, const msa_paged_batch* b,
+                                                       const msa_paged_attention_args* a) {
+  const int rc = check(c, b, a);
+  if (rc) return rc;
+  if (b->M == 0 || b->nseq == 0 || b->max_count == 0) return 0;
+  const Plan p = plan_of(*c, *b, *a);
+  return p.splits > 1 ? (int64_t)b->M * a->heads * p.splits * (c->hd + 4) * 4 : 0;
+}
+
+extern "C" int msa_paged_attention(const msa_paged_cache* c, const msa_paged_batch* b, const msa_paged_attention_args* a,
+                                   void* stream) {
+  const int rc = check(c, b, a);
+  if (rc) return rc;
+  if (b->M == 0 || b->nseq == 0 || b->max_count == 0) return MSA_OK;
+  const int64_t width = (int64_t)a->heads * c->hd;
+  MSA_REQUIRE(a->q && a->out, MSA_ERR_INVALID_ARG, "msa_paged_attention: null pointer");
+  MSA_REQUIRE(((uintptr_t)a->q | (uintptr_t)a->out | (uintptr_t)a->workspace) % 16 == 0, MSA_ERR_INVALID_ARG,
+              "msa_paged_attention: queries, outputs and workspace must be 16-byte aligned");
+  MSA_REQUIRE(a->ldq >= width && a->ldq % 8 == 0, MSA_ERR_INVALID_ARG, "msa_paged_attention: ldq must be a multiple of 8 of at least heads * hd");
+  if (a->out_mb > 0)
+    MSA_REQUIRE(c->dtype == MSA_F16 && b->M <= MSA_PACKED_MAX_ROWS && a->out_mb == packed_row_blocks(b->M) && width % 32 == 0,
+                MSA_ERR_INVALID_ARG, "msa_paged_attention: packed outputs are fp16, of at most 128 rows and a multiple of 32 columns");
+  else
+    MSA_REQUIRE(a->out_mb == 0 && a->ldo >= width && a->ldo % 8 == 0, MSA_ERR_INVALID_ARG,
+                "msa_paged_attention: ldo must be a multiple of 8 of at least heads * hd");
+  const int64_t need = msa_paged_attention_workspace_bytes(c, b, a);
+  MSA_REQUIRE(need == 0 || (a->workspace && a->workspace_bytes >= need), MSA_ERR_INVALID_ARG,
+              "msa_paged_attention: the workspace has %lld bytes, %lld are needed", (long long)a->workspace_bytes, (long long)need);
+  const Plan p = plan_of(*c, *b, *a);
+  MSA_REQUIRE((int64_t)b->nseq * p.row_blocks <= INT32_MAX, MSA_ERR_INVALID_ARG, "msa_paged_attention: too many rows for one call");
+  PagedAttention k = {a->q, c->k_pages, c->v_pages, c->k_exp, c->v_exp, b->seq_start, b->seq_pos, b->table, a->ldq, a->ldo,
+                      b->table_stride, a->out, (float*)a->workspace, b->M, b->nseq, a->heads, c->kv_heads, c->pages,
+                      paged_log2(c->page), b->blocks, a->out_mb, a->window, a->sinks, p.splits, p.row_blocks,
+                      c->dtype == MSA_BF16, b->max_count, a->scale};
+  hipStream_t s = (hipStream_t)stream;
+  switch (paged_format(*c)) {
+    case PG_F16: msa_launch_paged_rows_f16(k, c->hd, p.row_tiles, s); break;
+    case PG_BF16: msa_launch_paged_rows_bf16(k, c->hd, p.row_tiles, s); break;
+    case PG_E4M3: msa_launch_paged_rows_e4m3(k, c->hd, p.row_tiles, s); break;
+    default: msa_launch_paged_rows_i8(k, c->hd, p.row_tiles, s); break;
+  }
+  MSA_CHECK_LAUNCH("msa_paged_attention");
+  if (p.splits > 1) {
+    hipLaunchKernelGGL(paged_combine_kernel, dim3((unsigned)b->M, (unsigned)a->heads), dim3(64), 0, s, k, c->hd);
+    MSA_CHECK_LAUNCH("msa_paged_attention (splits)");
+  }
+  return MSA_OK;
+}

@@ -1,0 +1,6 @@
+// Attention over pages, few rows per sequence, bf16 pages
+#include "paged_attention.h"
+
+void msa_launch_paged_rows_bf16(const PagedAttention& a, int hd, int row_tiles, hipStream_t stream) {
+  pa_launch_rows_of<PG_BF16>(a, hd, row_tiles, stream);
+}

@@ -1,0 +1,6 @@
+// Attention over pages, few rows per sequence, int8 pages
+#include "paged_attention.h"
+
+void msa_launch_paged_rows_i8(const PagedAttention& a, int hd, int row_tiles, hipStream_t stream) {
+  pa_launch_rows_of<PG_I8>(a, hd, row_tiles, stream);
+}

@@ -1,0 +1,216 @@
+"""Keys and values of one attention layer in pages, as they are or in 8 bits, and the attention that reads them.
+
+The reference appends to one tensor per layer and re-copies the history at every step
+(metaseq/modules/multihead_attention.py:449-479); ``KVCache`` reserves a row of a fixed capacity per sequence.  Here
+a sequence's positions lie in pages of 16 to 256 positions that a table names in order, so that sequences of any length
+share one pool, several of them may share the pages of a common beginning, and pages that no window sees any more can be given
+to others.
+
+Layouts (contiguous): ``k_pages`` [pages, kv_heads, page, head_dim], ``v_pages`` [pages, kv_heads, head_dim, page].
+Their dtype is the format: fp16 or bf16 (that of keys, values, queries and outputs), or float8_e4m3fn or int8, whose codes c
+stand for c 2^e with one exponent e per position and head, ``k_exp`` and ``v_exp`` (int8 [pages, kv_heads, page]).
+"""
+import ctypes
+import math
+
+import torch
+
+from . import _capi
+from .decoder_base import upload
+
+PAGE_SIZES = (16, 32, 64, 128, 256)
+HEAD_DIMS = (64, 80, 96, 128, 192, 256)
+_DTYPES = {torch.float16: _capi.MSA_F16, torch.bfloat16: _capi.MSA_BF16}
+_FORMATS = {torch.float8_e4m3fn: _capi.MSA_PAGES_E4M3, torch.int8: _capi.MSA_PAGES_INT8}
+
+
+class PagedBatch:
+    """The new tokens of several sequences, one sequence's rows behind the other's (``PagedCache.batch``).
+
+    ``rows``: how many there are.  ``seq_start``, ``seq_pos``, ``table``: what the kernels read (int32, device);
+    ``seq_pos`` and ``table`` may be written between calls, on the stream that the calls run on - a captured graph
+    follows them - as long as no position reaches ``key_bound``."""
+
+    def __init__(self, c, rows, seq_start, seq_pos, table):
+        self.c, self.rows, self.seq_start, self.seq_pos, self.table = c, rows, seq_start, seq_pos, table
+        self.by_ref = ctypes.byref(c)
+
+    @property
+    def key_bound(self):
+        return self.c.key_bound
+
+
+class PagedCache:
+    """The pages of one layer.  The tensors are used as they are, not copied."""
+
+    def __init__(self, k_pages, v_pages, k_exp=None, v_exp=None):
+        if k_pages.dim() != 4:
+            raise ValueError("k_pages must be [pages, kv_heads, page, head_dim]")
+        pages, kv_heads, page, hd = k_pages.shape
+        eight = k_pages.dtype in _FORMATS
+        if not eight and k_pages.dtype not in _DTYPES:
+            raise ValueError("pages are fp16, bf16, float8_e4m3fn or int8, not %s" % k_pages.dtype)
+        if page not in PAGE_SIZES or hd not in HEAD_DIMS:
+            raise ValueError("pages of %d positions and heads of %d: pages of %s and heads of %s are supported"
+                             % (page, hd, PAGE_SIZES, HEAD_DIMS))
+        wanted = [("v_pages", v_pages, (pages, kv_heads, hd, page), k_pages.dtype)]
+        if eight:
+            wanted += [(n, t, (pages, kv_heads, page), torch.int8) for n, t in (("k_exp", k_exp), ("v_exp", v_exp))]
+        elif k_exp is not None or v_exp is not None:
+            raise ValueError("16-bit pages have no exponents")
+        for name, t, shape, dtype in wanted:
+            if t is None or tuple(t.shape) != shape or t.dtype != dtype or t.device != k_pages.device:
+                raise ValueError("%s must be %s %s on %s" % (name, dtype, list(shape), k_pages.device))
+        for t in (k_pages, v_pages, k_exp, v_exp):
+            if t is not None and not t.is_contiguous():
+                raise ValueError("pages and exponents must be contiguous")
+        if not k_pages.is_cuda:
+            raise RuntimeError("metaseq_amd: pages must live on the GPU (no CPU path exists)")
+        self.k_pages, self.v_pages, self.k_exp, self.v_exp = k_pages, v_pages, k_exp, v_exp
+        self.pages, self.kv_heads, self.page, self.head_dim = pages, kv_heads, page, hd
+        self.device = k_pages.device
+        self._lib = _capi.load()
+        self._c = {}
+        for dtype, code in _DTYPES.items():
+            if eight or dtype == k_pages.dtype:
+                c = _capi.PagedCacheC(code, _FORMATS.get(k_pages.dtype, _capi.MSA_PAGES_SAME), kv_heads, hd, page, pages,
+                                      *(_capi.ptr(t) for t in (k_pages, v_pages, k_exp, v_exp)))
+                self._c[dtype] = (c, ctypes.byref(c))
+
+    @classmethod
+    def empty(cls, pages, kv_heads, head_dim, page=64, dtype=torch.float16, device="cuda"):
+        """A cache of that many pages of ``dtype`` (float16, bfloat16, float8_e4m3fn or int8)."""
+        new = lambda *shape, dtype=dtype: torch.empty(shape, dtype=dtype, device=device)  # noqa: E731
+        exps = [new(pages, kv_heads, page, dtype=torch.int8) for _ in range(2)] if dtype in _FORMATS else []
+        return cls(new(pages, kv_heads, page, head_dim), new(pages, kv_heads, head_dim, page), *exps)
+
+    def bytes(self):
+        return sum(t.numel() * t.element_size() for t in (self.k_pages, self.v_pages, self.k_exp, self.v_exp)
+                   if t is not None)
+
+    # ------------------------------------------------------------------ batches
+    def batch(self, new, positions, table, key_bound=None):
+        """``new``: how many tokens each sequence adds (host).  ``positions``: the position of each one's first (host
+        list, or int32 device tensor that the calls read when they run; negative: the sequence sits them out).
+        ``table``: int32 device tensor [sequences, blocks], the page of each page-full of positions; positions whose
+        entry names no page are not stored, read as zeros and seen by no row.  ``key_bound``: no position reaches it
+        (default: from ``positions``, or what the table can name)."""
+        new = [int(n) for n in new]
+        if any(n < 0 for n in new):
+            raise ValueError("a negative number of new tokens")
+        if table.dim() != 2 or table.dtype != torch.int32 or table.device != self.device or table.shape[0] != len(new) \
+                or table.shape[1] < 1 or (table.shape[1] > 1 and table.stride(1) != 1) \
+                or (table.shape[0] > 1 and table.stride(0) < table.shape[1]):
+            raise ValueError("table must be int32 [%d, blocks] on %s with its rows apart" % (len(new), self.device))
+        span = table.shape[1] * self.page
+        start = [0]
+        for n in new:
+            start.append(start[-1] + n)
+        if torch.is_tensor(positions):
+            if positions.dtype != torch.int32 or tuple(positions.shape) != (len(new),) or positions.device != self.device \
+                    or (len(new) > 1 and positions.stride(0) != 1):
+                raise ValueError("positions must be int32 [%d] on %s" % (len(new), self.device))
+            seq_start, seq_pos, bound = upload(start, torch.int32, self.device), positions, span
+        else:
+            positions = [int(p) for p in positions]
+            if len(positions) != len(new):
+                raise ValueError("one position per sequence")
+            ends = [p + n for p, n in zip(positions, new) if p >= 0]
+            bound = max(ends, default=0)
+            if bound > span:
+                raise ValueError("position %d lies behind the %d that the table can name" % (bound - 1, span))
+            both = upload(start + positions, torch.int32, self.device)
+            seq_start, seq_pos = both[:len(start)], both[len(start):]
+        if key_bound is not None:
+            bound = int(key_bound)
+        stride = table.stride(0) if table.shape[0] > 1 else table.shape[1]
+        c = _capi.PagedBatchC(start[-1], len(new), max(new, default=0), max(0, min(bound, span)), table.shape[1], stride,
+                              seq_start.data_ptr(), seq_pos.data_ptr(), table.data_ptr())
+        return PagedBatch(c, start[-1], seq_start, seq_pos, table)
+
+    # ------------------------------------------------------------------ calls
+    def _of(self, dtype):
+        if dtype not in self._c:
+            raise ValueError("pages of %s hold no %s" % (self.k_pages.dtype, dtype))
+        return self._c[dtype][1]
+
+    def _rows(self, name, t, rows, heads, copy):
+        """``t`` as rows of heads, one behind the other, that the kernels can read or write in place."""
+        if tuple(t.shape) != (rows, heads, self.head_dim) or t.device != self.device:
+            raise ValueError("%s must be [%d, %d, %d] on %s, not %s on %s"
+                             % (name, rows, heads, self.head_dim, self.device, list(t.shape), t.device))
+        _, sh, sd = t.stride()
+        if sd == 1 and (heads == 1 or sh == self.head_dim) and t.data_ptr() % 16 == 0 and \
+                (rows < 2 or (t.stride(0) % 8 == 0 and t.stride(0) >= heads * self.head_dim)):
+            return t
+        if not copy:
+            raise ValueError("%s must have its heads one behind the other, 16-byte aligned, rows a multiple of 8 apart"
+                             % name)
+        return t.contiguous() if not t.is_contiguous() else t.clone()
+
+    @staticmethod
+    def _ld(t):
+        return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+    def _run(self, fn, *args):
+        if torch.cuda.current_device() == self.device.index:
+            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+        else:
+            with torch.cuda.device(self.device):
+                rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+        if rc:
+            _capi.check(rc, self._lib)
+
+    def append(self, batch, k, v):
+        """Stores the keys and values ([rows, kv_heads, head_dim], fp16 or bf16, any row stride) of a batch's tokens at
+        their positions."""
+        if k.dtype != v.dtype:
+            raise ValueError("keys are %s, values %s" % (k.dtype, v.dtype))
+        c = self._of(k.dtype)
+        k = self._rows("k", k, batch.rows, self.kv_heads, True)
+        v = self._rows("v", v, batch.rows, self.kv_heads, True)
+        self._run(self._lib.msa_paged_append, c, batch.by_ref, k.data_ptr(), self._ld(k), v.data_ptr(), self._ld(v))
+
+    def read(self, batch, dtype=None, out=None):
+        """Keys and values at the positions of a batch's tokens, ([rows, kv_heads, head_dim],) * 2 of ``dtype`` (8-bit
+        pages; default fp16).  ``out``: a pair of tensors to write them to; rows of sequences that sit the call out, and rows
+        behind the last sequence's, keep what they hold there."""
+        if out is None:
+            dtype = dtype or (torch.float16 if self.k_pages.dtype in _FORMATS else self.k_pages.dtype)
+            shape = (batch.rows, self.kv_heads, self.head_dim)
+            out = tuple(torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
+        elif out[0].dtype != out[1].dtype or dtype not in (None, out[0].dtype):
+            raise ValueError("keys and values come in one dtype")
+        c = self._of(out[0].dtype)
+        k, v = (self._rows("out", t, batch.rows, self.kv_heads, False) for t in out)
+        self._run(self._lib.msa_paged_read, c, batch.by_ref, k.data_ptr(), self._ld(k), v.data_ptr(), self._ld(v))
+        return out
+
+    def attend(self, batch, q, *, scale=None, window=0, sinks=0, out=None):
+        """Attention of a batch's tokens, whose keys and values are stored already: ``q`` [rows, heads, head_dim], the
+        output alike.  A token at position i sees positions j <= i; with ``window`` only those with j > i - window or
+        j < ``sinks``.  ``scale``: default head_dim ** -0.5.  Rows of sequences that sit the call out keep what ``out``
+        holds (or are undefined)."""
+        if q.dim() != 3 or q.shape[1] % self.kv_heads or q.shape[1] == 0:
+            raise ValueError("q must be [rows, heads, head_dim], heads a multiple of %d" % self.kv_heads)
+        c = self._of(q.dtype)
+        heads = q.shape[1]
+        q = self._rows("q", q, batch.rows, heads, True)
+        if out is None:
+            out = torch.empty(batch.rows, heads, self.head_dim, dtype=q.dtype, device=self.device)
+        elif out.dtype != q.dtype:
+            raise ValueError("out must be %s" % q.dtype)
+        else:
+            self._rows("out", out, batch.rows, heads, False)
+        a = _capi.PagedAttentionArgs(heads, q.data_ptr(), self._ld(q), out.data_ptr(), self._ld(out), 0, window, sinks,
+                                     1.0 / math.sqrt(self.head_dim) if scale is None else scale, None, 0)
+        ref = ctypes.byref(a)
+        need = self._lib.msa_paged_attention_workspace_bytes(c, batch.by_ref, ref)
+        if need < 0:
+            _capi.check(need, self._lib)
+        if need:
+            # (from torch's allocator, so that two captured graphs never share one)
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), need
+        self._run(self._lib.msa_paged_attention, c, batch.by_ref, ref)
+        return out
