@@ -24,6 +24,8 @@ struct PagedAttention {
   void* out;
   float* partial;  // splits > 1: [M][heads][splits][hd + 4]
   int M, nseq, heads, kv_heads, pages, page_log2, blocks, out_mb, window, sinks, splits, row_blocks, bf16, max_count;
+  int few;      // sequences of at most so many (token, query head) rows of a key/value head are the wave kernel's
+  int grouped;  // tile kernel: all workgroups of a (sequence, head) on one XCD
   float scale;
 };
 

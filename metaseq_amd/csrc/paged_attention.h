@@ -17,6 +17,8 @@
 
 #include <math.h>
 
+#include <atomic>
+
 #include "paged.h"
 
 namespace {
@@ -34,6 +36,17 @@ struct PaFormat {
   static constexpr int NT = KT / 16;           // 16-key tiles of S^T in it
   static constexpr float SHIFT = F == PG_BF16 ? 0.f : 10.f;
 };
+
+// allows a kernel that much dynamic LDS, once per device (`done`: one bit each)
+bool pa_raise_lds(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return false;
+  const uint64_t bit = 1ull << dev;
+  if (done.load(std::memory_order_acquire) & bit) return true;
+  if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return false;
+  done.fetch_or(bit, std::memory_order_release);
+  return true;
+}
 
 __device__ __forceinline__ half8_t pa_e4m3(uint32_t lo, uint32_t hi) {
   const half2_t a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true);
@@ -155,7 +168,7 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
   const int row0 = a.seq_start[s], pos = a.seq_pos[s];
   int count = min(a.seq_start[s + 1], a.M) - row0;
   count = min(count, a.max_count);
-  if (pos < 0 || row0 < 0 || count <= 0 || rb * 16 * RT >= count * group) return;
+  if (pos < 0 || row0 < 0 || count <= 0 || count * group > a.few || rb * 16 * RT >= count * group) return;
   const int page = 1 << a.page_log2, rows = count * group, rho0 = rb * 16 * RT;
   const int limit = a.blocks * page - 1;  // last position that can be anywhere
   const int p_lo = (int)min((int64_t)pos + rho0 / group, (int64_t)limit);
@@ -452,6 +465,455 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
   }
 }
 
+// ---- portions of prompts: more than PA_FEW rows (token, query head) of a key/value head in a sequence ----------------
+// Workgroup = 128 rows, 4 waves of 32; tiles of 64 keys go through LDS, two of keys and two of values, one barrier a
+// tile.  Everything transposed as above, with v_mfma 32x32x16: a lane has row n = lane % 32 and, with hl = lane / 32, 16 of 32
+// keys.  Row m of a block of S^T stands for the key with bits 2 and 3 of m exchanged, so that the eight probabilities
+// of a step of the product with V belong to eight consecutive keys: one 128-bit read of the transposed values.
+// 16-bit pages go to LDS directly (global_load_lds_dwordx4: 16 bytes a lane to consecutive places, from anywhere), 8-bit
+// ones through registers, where they become fp16: keys times 2^(e - the tile's largest e), values times 2^(e - E), E the largest so
+// far.  Chunks of 16 bytes of a row are exchanged by the row's number, so that reads of many rows meet all banks.
+constexpr int PT_BM = 128, PT_BN = 64, PT_THREADS = 256;
+constexpr int PA_FEW = 32;  // rows that the wave kernel above takes
+
+typedef __attribute__((address_space(3))) void pt_lds_void;
+
+// where chunk c of row `row` of a tile with CH chunks to a row stands in that row
+template <int CH>
+__device__ __forceinline__ int pt_place(int c, int row) {
+  if (CH % 16 == 0) return c ^ (row & 15);
+  if (CH % 8 == 0) return c ^ ((row >> 1) & 7);
+  const int p = c + (CH == 12 ? (row >> 2) & 3 : (row >> 3) & 1);  // 12, 10: 192, 160 bytes
+  return p >= CH ? p - CH : p;
+}
+template <int CH>
+__device__ __forceinline__ int pt_chunk_at(int p, int row) {  // the chunk that stands at place p
+  if (CH % 8 == 0) return pt_place<CH>(p, row);
+  const int c = p - (CH == 12 ? (row >> 2) & 3 : (row >> 3) & 1);
+  return c < 0 ? c + CH : c;
+}
+
+template <int F>
+__device__ __forceinline__ float16_t pt_mfma(pg_u4 a, pg_u4 b, float16_t c) {
+  if (F == PG_BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+}
+
+template <int F, int HD>
+__global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kernel(PagedAttention a) {
+  typedef PaFormat<F> X;
+  constexpr bool B8 = X::bits8;
+  constexpr int ES = X::ES;
+  constexpr int KSTEPS = HD / 16, DBLK = (HD + 31) / 32;
+  constexpr int CH = HD / 8;                    // 16-byte chunks of a key row in LDS, which holds 16-bit elements
+  constexpr int ROWB = HD * 2, TILEB = PT_BN * ROWB;
+  constexpr int NI = TILEB / 1024;              // direct load instructions of a tile
+  constexpr float SHIFT = X::SHIFT;
+  extern __shared__ __attribute__((aligned(16))) char lds[];  // K, K, V, V
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n32 = lane & 31, hl = lane >> 5;
+  const int group = a.heads / a.kv_heads;
+  // workgroup -> (sequence, key/value head), row block, split: see the launch
+  int unit_id, rest;
+  if (a.grouped) {
+    const int j = blockIdx.x >> 3, per = a.row_blocks * a.splits;
+    unit_id = (j / per) * 8 + (blockIdx.x & 7);
+    rest = j % per;
+  } else {
+    const int units = a.nseq * a.kv_heads;
+    rest = blockIdx.x / units;
+    unit_id = blockIdx.x - rest * units;
+  }
+  const int split = rest % a.splits, rb = a.row_blocks - 1 - rest / a.splits;
+  const int s = unit_id / a.kv_heads, h = unit_id - s * a.kv_heads;
+  if (s >= a.nseq) return;
+  const int row0 = a.seq_start[s], pos = a.seq_pos[s];
+  const int count = min(min(a.seq_start[s + 1], a.M) - row0, a.max_count);
+  if (pos < 0 || row0 < 0 || count <= 0 || count * group <= a.few || rb * PT_BM >= count * group) return;
+  const int page = 1 << a.page_log2, rows = count * group, rho0 = rb * PT_BM;
+  const int limit = a.blocks * page - 1;
+  auto position = [&](int rho) { return (int)min((int64_t)pos + min(rho, rows - 1) / group, (int64_t)limit); };
+  const PaTiles<PT_BN> tiles(position(rho0), position(rho0 + PT_BM - 1), a.window, a.sinks);
+  const int per = (tiles.n + a.splits - 1) / a.splits;
+  const int it0 = split * per, it_end = min(tiles.n, it0 + per);
+  // of this wave
+  const int w0 = rho0 + wave * 32;
+  const int p_lo = position(w0), p_hi = position(w0 + 31);
+
+  // ---- queries: B operand, row n32, 8 dimensions at 16 ks + 8 hl ----
+  const int rho = w0 + n32;
+  const bool live = rho < rows;
+  const int tok = live ? rho / group : 0, g = live ? rho - tok * group : 0;
+  const int pn = live ? position(rho) : -1;
+  pg_u4 qf[KSTEPS];
+  float qs = a.scale * PA_LOG2E;
+  {
+    const char* q = (const char*)a.q + (((int64_t)row0 + tok) * a.ldq + (int64_t)(h * group + g) * HD + hl * 8) * 2;
+#pragma unroll
+    for (int ks = 0; ks < KSTEPS; ++ks) qf[ks] = *(const pg_u4*)(q + ks * 32);
+    if (B8 && a.bf16) {
+      float big = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KSTEPS; ++ks) {
+        const bf16x8_t v = __builtin_bit_cast(bf16x8_t, qf[ks]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf((float)v[i]));
+      }
+      big = fmaxf(big, __shfl_xor(big, 32, MSA_WAVE));
+      const int k = min(max((int)(__builtin_bit_cast(uint32_t, big) >> 23) - 127 - 8, -118), 120);
+#pragma unroll
+      for (int ks = 0; ks < KSTEPS; ++ks) {
+        const bf16x8_t v = __builtin_bit_cast(bf16x8_t, qf[ks]);
+        half8_t w;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = (half_t)ldexpf((float)v[i], -k);
+        qf[ks] = __builtin_bit_cast(pg_u4, w);
+      }
+      qs = ldexpf(qs, k);
+    }
+  }
+
+  // ---- tiles ----
+  const int32_t* table = a.table + (int64_t)s * a.table_stride;
+  // page of the sixteen keys g16 of tile i, -1 where there is none
+  auto look = [&](int i, int g16) {
+    const int block = (tiles.tile(i) * PT_BN + g16 * 16) >> a.page_log2;
+    const int pg = block < a.blocks ? table[block] : -1;
+    return pg >= 0 && pg < a.pages ? pg : -1;
+  };
+  const int64_t unit = (int64_t)page * HD * ES;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(pt_lds_void*)lds;
+  // 16 bits: instruction u of the tile (every fourth is this wave's) fills 64 consecutive places
+  auto issue = [&](int i, int slot, const int (&pg)[4]) {
+    const int key0 = tiles.tile(i) * PT_BN;
+#pragma unroll
+    for (int u = 0; u < (NI + 3) / 4; ++u) {
+      const int n = u * 4 + wave;
+      if (NI % 4 != 0 && n >= NI) break;
+      {
+        const int at = n * 64 + lane, row = at / CH, c = pt_chunk_at<CH>(at % CH, row);
+        const int p = row < 32 ? (row < 16 ? pg[0] : pg[1]) : (row < 48 ? pg[2] : pg[3]);
+        const char* from = (const char*)a.k_pages + ((int64_t)max(p, 0) * a.kv_heads + h) * unit +
+                           (int64_t)((key0 + row) & (page - 1)) * ROWB + c * 16;
+        const uint32_t la = lds0 + slot * TILEB + n * 1024;
+        asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(la) : "memory");
+      }
+      {
+        const int at = n * 64 + lane, row = at / 8, c = pt_chunk_at<8>(at % 8, row), key = key0 + c * 8;
+        const int p = c < 4 ? (c < 2 ? pg[0] : pg[1]) : (c < 6 ? pg[2] : pg[3]);
+        const char* from = (const char*)a.v_pages + ((int64_t)max(p, 0) * a.kv_heads + h) * unit +
+                           ((int64_t)row * page + (key & (page - 1))) * 2;
+        const uint32_t la = lds0 + (2 + slot) * TILEB + n * 1024;
+        asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(la) : "memory");
+      }
+    }
+  };
+  // whether any row of the workgroup sees the key
+  const int g_lo = position(rho0), g_hi = position(rho0 + PT_BM - 1);
+  auto anyone = [&](int key) { return key <= g_hi && (a.window <= 0 || key > g_lo - a.window || key < a.sinks); };
+  // 8 bits: chunks of 16 elements, registers in between
+  constexpr int CB = HD / 16, KN = (PT_BN * CB + PT_THREADS - 1) / PT_THREADS, VN = (HD * 4 + PT_THREADS - 1) / PT_THREADS;
+  pg_u4 kr[B8 ? KN : 1], vr[B8 ? VN : 1], vx;
+  int kx[B8 ? KN : 1], ke = 0, ve = 0;  // the rows' exponents; those of key `lane` of the tile
+  const int vg = threadIdx.x & 3;       // the sixteen keys that the thread's chunks of V belong to
+  auto fetch = [&](int i, const int (&pg)[4]) {
+    const int key0 = tiles.tile(i) * PT_BN;
+    auto page_of = [&](int g16) { return g16 < 2 ? (g16 < 1 ? pg[0] : pg[1]) : (g16 < 3 ? pg[2] : pg[3]); };
+#pragma unroll
+    for (int j = 0; j < KN; ++j) {
+      const int at = min((int)threadIdx.x + j * PT_THREADS, PT_BN * CB - 1), row = at / CB, c = at % CB;
+      const int64_t up = ((int64_t)max(page_of(row >> 4), 0) * a.kv_heads + h) * page + ((key0 + row) & (page - 1));
+      kr[j] = *(const pg_u4*)((const char*)a.k_pages + up * HD + c * 16);
+      kx[j] = a.k_exp[up];
+    }
+    const int64_t uv = (int64_t)max(page_of(vg), 0) * a.kv_heads + h;
+    const int in = (key0 + vg * 16) & (page - 1);
+#pragma unroll
+    for (int j = 0; j < VN; ++j) {
+      const int row = min((int)threadIdx.x + j * PT_THREADS, HD * 4 - 1) >> 2;
+      vr[j] = *(const pg_u4*)((const char*)a.v_pages + uv * unit + (int64_t)row * page + in);
+    }
+    vx = *(const pg_u4*)(a.v_exp + uv * page + in);
+    const int64_t ul = ((int64_t)max(page_of(lane >> 4), 0) * a.kv_heads + h) * page + ((key0 + lane) & (page - 1));
+    ke = a.k_exp[ul];
+    ve = a.v_exp[ul];
+  };
+  auto wave_most = [](int v) { return (int)wave_max((float)v); };
+  // (returns the exponents that the tile's keys and values are relative to)
+  auto stage = [&](int i, int slot, const int (&pg)[4], int& ek, int& ev) {
+    const int key0 = tiles.tile(i) * PT_BN;
+    auto page_of = [&](int g16) { return g16 < 2 ? (g16 < 1 ? pg[0] : pg[1]) : (g16 < 3 ? pg[2] : pg[3]); };
+    const bool mine = page_of(lane >> 4) >= 0 && anyone(key0 + lane);
+    ek = __builtin_amdgcn_readfirstlane(wave_most(mine ? ke : -127));
+    ev = max(ev, __builtin_amdgcn_readfirstlane(wave_most(mine ? ve : -127)));
+    char* kt = lds + slot * TILEB;
+    char* vt = lds + (2 + slot) * TILEB;
+    auto power = [](int e) { return ldexpf(1.f, min(max(e, -126), 0)); };
+#pragma unroll
+    for (int j = 0; j < KN; ++j) {
+      const int at = threadIdx.x + j * PT_THREADS, row = at / CB, c = at % CB;
+      if ((PT_BN * CB) % PT_THREADS == 0 || at < PT_BN * CB) {
+        const half_t f = (half_t)power(kx[j] - ek);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          half8_t w = __builtin_bit_cast(half8_t, pa_operand<F>(kr[j], e));
+          w *= f;
+          *(half8_t*)(kt + row * ROWB + pt_place<CH>(2 * c + e, row) * 16) = w;
+        }
+      }
+    }
+    half8_t f[2];
+    pg_u4 keep;
+    const bool there = page_of(vg) >= 0;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const bool sees = there && anyone(key0 + vg * 16 + k);
+      f[k >> 3][k & 7] = (half_t)(sees ? power((int)(int8_t)(vx[k >> 2] >> ((k & 3) * 8)) - ev) : 0.f);
+      keep[k >> 2] = ((k & 3) ? keep[k >> 2] : 0) | (sees ? 0xffu << ((k & 3) * 8) : 0);
+    }
+#pragma unroll
+    for (int j = 0; j < VN; ++j) {
+      const int at = threadIdx.x + j * PT_THREADS, row = at >> 2;
+      if ((HD * 4) % PT_THREADS == 0 || at < HD * 4) {
+        const pg_u4 w = vr[j] & keep;
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          *(half8_t*)(vt + row * 128 + pt_place<8>(2 * vg + e, row) * 16) = __builtin_bit_cast(half8_t, pa_operand<F>(w, e)) * f[e];
+      }
+    }
+  };
+
+  // ---- fragments: K block ib, step ks: row with bits 2 and 3 of n32 exchanged, chunk 2 ks + hl.  V^T block db, step c (16
+  // keys): row 32 db + n32, chunk 2 c + hl ----
+  const int krow = (n32 & ~12) | ((n32 & 4) << 1) | ((n32 & 8) >> 1);
+  float16_t o[DBLK];
+#pragma unroll
+  for (int d = 0; d < DBLK; ++d)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) o[d][v] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  int E = -127, ek[2] = {0, 0}, ev[2] = {-127, -127};
+  int pg[2][4];  // pages of the tile at hand and the next one's
+  auto look4 = [&](int i, int (&p)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) p[k] = look(min(i, it_end - 1), k);
+  };
+  if (it0 < it_end) {
+    look4(it0, pg[0]);
+    look4(it0 + 1, pg[1]);
+    if (B8) {
+      fetch(it0, pg[0]);
+      stage(it0, 0, pg[0], ek[0], ev[0]);
+    } else {
+      issue(it0, 0, pg[0]);
+    }
+  }
+  for (int i = it0; i < it_end; ++i) {
+    const int slot = (i - it0) & 1;
+    const int here = (pg[0][0] >= 0 ? 1 : 0) | (pg[0][1] >= 0 ? 2 : 0) | (pg[0][2] >= 0 ? 4 : 0) | (pg[0][3] >= 0 ? 8 : 0);
+    if (!B8) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();  // the tile is complete, and the other slots are free
+    if (i + 1 < it_end) {
+      if (B8) fetch(i + 1, pg[1]);
+      else issue(i + 1, slot ^ 1, pg[1]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) pg[0][k] = pg[1][k];
+    if (i + 2 < it_end) look4(i + 2, pg[1]);
+
+    const char* kt = lds + slot * TILEB;
+    const char* vt = lds + (2 + slot) * TILEB;
+    const int key0 = tiles.tile(i) * PT_BN;
+    const bool whole = key0 + PT_BN - 1 <= p_lo && (a.window <= 0 || key0 > p_hi - a.window || key0 + PT_BN <= a.sinks) && here == 15;
+    // (a wave whose rows see nothing of the tile has nothing to do)
+    const bool none = key0 > p_hi || w0 >= rows || (a.window > 0 && key0 + PT_BN - 1 <= p_lo - a.window && key0 >= a.sinks);
+    if (!none) {
+      float16_t sc[2];
+#pragma unroll
+      for (int ib = 0; ib < 2; ++ib)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) sc[ib][v] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KSTEPS; ++ks)
+#pragma unroll
+        for (int ib = 0; ib < 2; ++ib) {
+          const int row = ib * 32 + krow;
+          const pg_u4 k = *(const pg_u4*)(kt + row * ROWB + pt_place<CH>(2 * ks + hl, row) * 16);
+          sc[ib] = pt_mfma<F>(k, qf[ks], sc[ib]);
+        }
+      const float c = B8 ? ldexpf(qs, ek[slot]) : qs;
+      // key of element v of block ib
+      auto key_of = [&](int ib, int v) { return key0 + ib * 32 + (v >> 3) * 16 + hl * 8 + (v & 7); };
+      float top = -INFINITY;
+      if (whole) {
+#pragma unroll
+        for (int ib = 0; ib < 2; ++ib)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) top = fmaxf(top, sc[ib][v]);
+      } else {
+#pragma unroll
+        for (int ib = 0; ib < 2; ++ib)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const int key = key_of(ib, v);
+            if (!(here >> (ib * 2 + (v >> 3)) & 1) || key > pn || (a.window > 0 && key <= pn - a.window && key >= a.sinks))
+              sc[ib][v] = -INFINITY;
+            top = fmaxf(top, sc[ib][v]);
+          }
+      }
+      top *= c;
+      if (B8 && ev[slot] > E) {
+#pragma unroll
+        for (int d = 0; d < DBLK; ++d)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) o[d][v] = ldexpf(o[d][v], E - ev[slot]);
+        E = ev[slot];
+      }
+      if (__ballot(top > m + PA_LAZY)) {
+        const float to = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, MSA_WAVE)));
+        const float w = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - to);
+        m = to;
+        l *= w;
+#pragma unroll
+        for (int d = 0; d < DBLK; ++d)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) o[d][v] *= w;
+      }
+      const float off = (m == -INFINITY ? 0.f : m) - SHIFT;
+      pg_u4 p[4];  // step 2 ib + c of the product with V
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int ib = 0; ib < 2; ++ib)
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+          float e[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[ib][cc * 8 + j], c, -off));
+            sum[j & 1] += e[j];
+          }
+          if (F == PG_BF16) {
+            bf16x8_t w;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = (bf16_t)e[j];
+            p[ib * 2 + cc] = __builtin_bit_cast(pg_u4, w);
+          } else {
+            half8_t w;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = (half_t)e[j];
+            p[ib * 2 + cc] = __builtin_bit_cast(pg_u4, w);
+          }
+        }
+      l += sum[0] + sum[1];
+      auto v_at = [&](int db, int st) {
+        const int row = HD % 32 == 0 ? db * 32 + n32 : min(db * 32 + n32, HD - 1);
+        return *(const pg_u4*)(vt + row * 128 + pt_place<8>(2 * st + hl, row) * 16);
+      };
+      if (whole) {
+#pragma unroll
+        for (int st = 0; st < 4; ++st)
+#pragma unroll
+          for (int db = 0; db < DBLK; ++db) o[db] = pt_mfma<F>(v_at(db, st), p[st], o[db]);
+      } else {
+        // as in the kernel above: values that no row sees are zeros, and those that are not finite reach the rows that
+        // see them only
+#pragma unroll
+        for (int st = 0; st < 4; ++st) {
+          uint32_t seen = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int key = key0 + st * 16 + hl * 8 + j;
+            const bool sees = (here >> st & 1) && key <= p_hi && (a.window <= 0 || key > p_lo - a.window || key < a.sinks);
+            seen |= sees ? 1u << j : 0;
+          }
+#pragma unroll
+          for (int db = 0; db < DBLK; ++db) {
+            constexpr int G = F == PG_BF16 ? PG_BF16 : PG_F16;  // LDS holds 16 bits in every format
+            pg_u4 v = v_at(db, st);
+            bool odd = false;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              v[k] = pa_keep<G>(v[k], seen >> (2 * k));
+              odd |= pa_not_finite<G>(v[k], 0) != 0;
+            }
+            if (__ballot(odd)) {
+#pragma unroll 1
+              for (int kind = 1; kind <= 3; ++kind) {
+                pg_u4 ones;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) ones[k] = pa_not_finite<G>(v[k], kind);
+                float16_t hit;
+#pragma unroll
+                for (int k = 0; k < 16; ++k) hit[k] = 0.f;
+                hit = pt_mfma<F>(ones, p[st], hit);
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                  if (hit[k] != 0.f) o[db][k] += kind == 1 ? INFINITY : kind == 2 ? -INFINITY : NAN;
+              }
+#pragma unroll
+              for (int k = 0; k < 4; ++k) v[k] = pa_finite<G>(v[k]);
+            }
+            o[db] = pt_mfma<F>(v, p[st], o[db]);
+          }
+        }
+      }
+    }
+    if (B8 && i + 1 < it_end) {
+      ev[slot ^ 1] = ev[slot];
+      stage(i + 1, slot ^ 1, pg[0], ek[slot ^ 1], ev[slot ^ 1]);
+    }
+  }
+
+  // ---- O^T: row n32, dimensions 32 db + 8 blk + 4 hl + r ----
+  l += __shfl_xor(l, 32, MSA_WAVE);
+  if (!live) return;
+  const int head = h * group + g;
+  const int64_t row = (int64_t)row0 + tok;
+  if (a.splits > 1) {
+    float* to = a.partial + ((row * a.heads + head) * a.splits + split) * (HD + 4);
+#pragma unroll
+    for (int db = 0; db < DBLK; ++db)
+#pragma unroll
+      for (int blk = 0; blk < 4; ++blk) {
+        const int d = db * 32 + blk * 8 + hl * 4;
+        float4_t v;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = B8 ? ldexpf(o[db][blk * 4 + r], E) : o[db][blk * 4 + r];
+        if (HD % 32 == 0 || d < HD) *(float4_t*)(to + d) = v;
+      }
+    if (hl == 0) to[HD] = m, to[HD + 1] = l;
+    return;
+  }
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll
+  for (int db = 0; db < DBLK; ++db)
+#pragma unroll
+    for (int blk = 0; blk < 4; ++blk) {
+      const int d = db * 32 + blk * 8 + hl * 4;
+      uint16_t w[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float z = (B8 ? ldexpf(o[db][blk * 4 + r], E) : o[db][blk * 4 + r]) * inv;
+        w[r] = a.bf16 ? __builtin_bit_cast(uint16_t, (bf16_t)z) : __builtin_bit_cast(uint16_t, (half_t)z);
+      }
+      const int64_t at = a.out_mb > 0 ? packed_act_offset((int)row, head * HD + d, a.out_mb) : row * a.ldo + head * HD + d;
+      if (HD % 32 == 0 || d < HD) *(pg_u2*)((uint16_t*)a.out + at) = pg_u2{(uint32_t)w[0] | (uint32_t)w[1] << 16, (uint32_t)w[2] | (uint32_t)w[3] << 16};
+    }
+}
+
+template <int F, int HD>
+bool pa_launch_tiles(const PagedAttention& a, hipStream_t stream) {
+  constexpr int bytes = 4 * PT_BN * HD * 2;
+  static std::atomic<uint64_t> done{0};
+  if (!pa_raise_lds((const void*)paged_tile_kernel<F, HD>, bytes, done)) return false;
+  const int64_t units = (int64_t)a.nseq * a.kv_heads, per = (int64_t)a.row_blocks * a.splits;
+  const int64_t n = a.grouped ? (units + 7) / 8 * 8 * per : units * per;
+  hipLaunchKernelGGL((paged_tile_kernel<F, HD>), dim3((unsigned)n), dim3(PT_THREADS), bytes, stream, a);
+  return true;
+}
+
 template <int F, int HD>
 void pa_launch_rows(const PagedAttention& a, int rt, hipStream_t stream) {
   const dim3 grid((unsigned)((int64_t)a.nseq * a.row_blocks), (unsigned)a.kv_heads, (unsigned)a.splits);
@@ -468,6 +930,18 @@ void pa_launch_rows_of(const PagedAttention& a, int hd, int rt, hipStream_t stre
     case 128: return pa_launch_rows<F, 128>(a, rt, stream);
     case 192: return pa_launch_rows<F, 192>(a, rt, stream);
     default: return pa_launch_rows<F, 256>(a, rt, stream);
+  }
+}
+
+template <int F>
+bool pa_launch_tiles_of(const PagedAttention& a, int hd, hipStream_t stream) {
+  switch (hd) {
+    case 64: return pa_launch_tiles<F, 64>(a, stream);
+    case 80: return pa_launch_tiles<F, 80>(a, stream);
+    case 96: return pa_launch_tiles<F, 96>(a, stream);
+    case 128: return pa_launch_tiles<F, 128>(a, stream);
+    case 192: return pa_launch_tiles<F, 192>(a, stream);
+    default: return pa_launch_tiles<F, 256>(a, stream);
   }
 }
 

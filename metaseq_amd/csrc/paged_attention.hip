@@ -1,25 +1,32 @@
 // Attention over pages: which kernel takes a batch, how keys are split, and the sum of the splits.
 #include "paged_attention.h"
 
-void msa_launch_paged_rows_f16(const PagedAttention& a, int hd, int row_tiles, hipStream_t stream);
-void msa_launch_paged_rows_bf16(const PagedAttention& a, int hd, int row_tiles, hipStream_t stream);
-void msa_launch_paged_rows_e4m3(const PagedAttention& a, int hd, int row_tiles, hipStream_t stream);
-void msa_launch_paged_rows_i8(const PagedAttention& a, int hd, int row_tiles, hipStream_t stream);
+#define PAGED_FORMAT(name)                                                                      \
+  void msa_launch_paged_rows_##name(const PagedAttention& a, int hd, int row_tiles, hipStream_t s); \
+  bool msa_launch_paged_tiles_##name(const PagedAttention& a, int hd, hipStream_t s);
+PAGED_FORMAT(f16)
+PAGED_FORMAT(bf16)
+PAGED_FORMAT(e4m3)
+PAGED_FORMAT(i8)
 
 namespace {
 
 // One wave per (row, query head): out = sum of the splits' sums, each relative to its own maximum.
-__global__ __launch_bounds__(64) void paged_combine_kernel(PagedAttention a, int hd) {
+// `few`, `many`: splits of the sequences of either kernel; 1: it wrote its outputs itself.
+__global__ __launch_bounds__(64) void paged_combine_kernel(PagedAttention a, int hd, int few, int many) {
   const int lane = threadIdx.x, r = blockIdx.x, head = blockIdx.y;
   const int s = __builtin_amdgcn_readfirstlane(paged_sequence_of(a.seq_start, a.nseq, r));
   if (s >= a.nseq || r >= a.seq_start[a.nseq] || a.seq_pos[s] < 0 || a.seq_start[s] < 0 || r - a.seq_start[s] >= a.max_count) return;
-  const float* part = a.partial + ((int64_t)r * a.heads + head) * a.splits * (hd + 4);
+  const int count = min(min(a.seq_start[s + 1], a.M) - a.seq_start[s], a.max_count);
+  const int splits = count * (a.heads / a.kv_heads) <= a.few ? few : many;
+  if (splits == 1) return;
+  const float* part = a.partial + ((int64_t)r * a.heads + head) * splits * (hd + 4);
   float top = -INFINITY;
-  for (int i = lane; i < a.splits; i += 64) top = fmaxf(top, part[(int64_t)i * (hd + 4) + hd]);
+  for (int i = lane; i < splits; i += 64) top = fmaxf(top, part[(int64_t)i * (hd + 4) + hd]);
   top = wave_max(top);
   const float off = top == -INFINITY ? 0.f : top;
   float o[4] = {0.f, 0.f, 0.f, 0.f}, total = 0.f;
-  for (int i = 0; i < a.splits; ++i) {
+  for (int i = 0; i < splits; ++i) {
     const float* p = part + (int64_t)i * (hd + 4);
     const float w = __builtin_amdgcn_exp2f(p[hd] - off);
     total += w * p[hd + 1];
@@ -38,26 +45,52 @@ __global__ __launch_bounds__(64) void paged_combine_kernel(PagedAttention a, int
   *(pg_u2*)((uint16_t*)a.out + at) = pg_u2{(uint32_t)w[0] | (uint32_t)w[1] << 16, (uint32_t)w[2] | (uint32_t)w[3] << 16};
 }
 
+// How a batch is taken: sequences of at most PA_FEW rows (token, query head) of a key/value head by the wave kernel, others
+// by tiles; each splits keys over workgroups where there are few of those.
 struct Plan {
-  int row_tiles, row_blocks, splits;
+  int row_tiles, row_blocks, splits;      // wave kernel (row_tiles 0: not launched)
+  int tile_blocks, tile_splits, grouped;  // tile kernel (tile_blocks 0: not launched)
 };
 
-Plan plan_of(const msa_paged_cache& c, const msa_paged_batch& b, const msa_paged_attention_args& a) {
-  Plan p;
-  const int64_t rows = (int64_t)b.max_count * (a.heads / c.kv_heads);
-  p.row_tiles = rows <= 16 ? 1 : 2;
-  p.row_blocks = (int)((rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
-  // keys that a row block can see, in tiles of the format; a split is at least one tile per wave
-  int64_t keys = b.key_bound;
-  if (a.window > 0) keys = keys < (int64_t)a.window + a.sinks + b.max_count ? keys : (int64_t)a.window + a.sinks + b.max_count;
-  const int kt = c.format == MSA_PAGES_SAME ? 32 : 64;
-  const int64_t tiles = (keys + kt - 1) / kt, groups = (int64_t)b.nseq * p.row_blocks * c.kv_heads;
-  const int64_t most = (tiles + PA_NW - 1) / PA_NW;
-  int64_t s = groups >= 512 ? 1 : 1024 / groups;
+int splits_of(int64_t groups, int64_t enough, int64_t tiles, int64_t least) {
+  const int64_t most = (tiles + least - 1) / least;
+  int64_t s = groups >= enough / 2 ? 1 : enough / groups;
   if (s > most) s = most;
   if (s > 128) s = 128;
-  p.splits = s < 1 ? 1 : (int)s;
+  return s < 1 ? 1 : (int)s;
+}
+
+Plan plan_of(const msa_paged_cache& c, const msa_paged_batch& b, const msa_paged_attention_args& a) {
+  Plan p = {0, 0, 1, 0, 1, 0};
+  const int group = a.heads / c.kv_heads;
+  const int64_t rows = (int64_t)b.max_count * group;
+  // whether every sequence has max_count rows
+  const bool even = (int64_t)b.nseq * b.max_count <= b.M;
+  // keys that a row block can see
+  auto keys_of = [&](int64_t tokens) {
+    const int64_t span = (int64_t)a.window + a.sinks + tokens;
+    return a.window > 0 && span < b.key_bound ? span : (int64_t)b.key_bound;
+  };
+  if (rows <= PA_FEW || !even) {
+    const int64_t most = rows < PA_FEW ? rows : PA_FEW;
+    p.row_tiles = most <= 16 ? 1 : 2;
+    p.row_blocks = (int)((most + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
+    const int kt = c.format == MSA_PAGES_SAME ? 32 : 64;
+    p.splits = splits_of((int64_t)b.nseq * p.row_blocks * c.kv_heads, 1024, (keys_of(most) + kt - 1) / kt, PA_NW);
+  }
+  if (rows > PA_FEW) {
+    p.tile_blocks = (int)((rows + PT_BM - 1) / PT_BM);
+    const int64_t units = (int64_t)b.nseq * c.kv_heads;
+    p.tile_splits = splits_of(units * p.tile_blocks, 512, (keys_of(PT_BM / group + 1) + PT_BN - 1) / PT_BN, 8);
+    p.grouped = units % 8 == 0 || units >= 64;
+  }
   return p;
+}
+
+// floats of one (row, head) in the workspace
+int64_t partial_floats(const Plan& p, int hd) {
+  const int64_t s = p.splits > p.tile_splits ? p.splits : p.tile_splits;
+  return s > 1 ? s * (hd + 4) : 0;
 }
 
 int check(const msa_paged_cache* c, const msa_paged_batch* b, const msa_paged_attention_args* a) {
@@ -79,8 +112,7 @@ extern "C" int64_t msa_paged_attention_workspace_bytes(const msa_paged_cache* c,
   const int rc = check(c, b, a);
   if (rc) return rc;
   if (b->M == 0 || b->nseq == 0 || b->max_count == 0) return 0;
-  const Plan p = plan_of(*c, *b, *a);
-  return p.splits > 1 ? (int64_t)b->M * a->heads * p.splits * (c->hd + 4) * 4 : 0;
+  return (int64_t)b->M * a->heads * partial_floats(plan_of(*c, *b, *a), c->hd) * 4;
 }
 
 extern "C" int msa_paged_attention(const msa_paged_cache* c, const msa_paged_batch* b, const msa_paged_attention_args* a,
@@ -103,21 +135,39 @@ extern "C" int msa_paged_attention(const msa_paged_cache* c, const msa_paged_bat
   MSA_REQUIRE(need == 0 || (a->workspace && a->workspace_bytes >= need), MSA_ERR_INVALID_ARG,
               "msa_paged_attention: the workspace has %lld bytes, %lld are needed", (long long)a->workspace_bytes, (long long)need);
   const Plan p = plan_of(*c, *b, *a);
-  MSA_REQUIRE((int64_t)b->nseq * p.row_blocks <= INT32_MAX, MSA_ERR_INVALID_ARG, "msa_paged_attention: too many rows for one call");
+  const int64_t units = (int64_t)b->nseq * c->kv_heads;
+  MSA_REQUIRE((int64_t)b->nseq * p.row_blocks <= INT32_MAX && (units + 7) * p.tile_blocks * p.tile_splits <= INT32_MAX,
+              MSA_ERR_INVALID_ARG, "msa_paged_attention: too many rows for one call");
   PagedAttention k = {a->q, c->k_pages, c->v_pages, c->k_exp, c->v_exp, b->seq_start, b->seq_pos, b->table, a->ldq, a->ldo,
                       b->table_stride, a->out, (float*)a->workspace, b->M, b->nseq, a->heads, c->kv_heads, c->pages,
-                      paged_log2(c->page), b->blocks, a->out_mb, a->window, a->sinks, p.splits, p.row_blocks,
-                      c->dtype == MSA_BF16, b->max_count, a->scale};
+                      paged_log2(c->page), b->blocks, a->out_mb, a->window, a->sinks, 1, 1,
+                      c->dtype == MSA_BF16, b->max_count, PA_FEW, p.grouped, a->scale};
   hipStream_t s = (hipStream_t)stream;
-  switch (paged_format(*c)) {
-    case PG_F16: msa_launch_paged_rows_f16(k, c->hd, p.row_tiles, s); break;
-    case PG_BF16: msa_launch_paged_rows_bf16(k, c->hd, p.row_tiles, s); break;
-    case PG_E4M3: msa_launch_paged_rows_e4m3(k, c->hd, p.row_tiles, s); break;
-    default: msa_launch_paged_rows_i8(k, c->hd, p.row_tiles, s); break;
+  const int format = paged_format(*c);
+  if (p.tile_blocks > 0) {
+    k.splits = p.tile_splits;
+    k.row_blocks = p.tile_blocks;
+    const bool ok = format == PG_F16    ? msa_launch_paged_tiles_f16(k, c->hd, s)
+                    : format == PG_BF16 ? msa_launch_paged_tiles_bf16(k, c->hd, s)
+                    : format == PG_E4M3 ? msa_launch_paged_tiles_e4m3(k, c->hd, s)
+                                        : msa_launch_paged_tiles_i8(k, c->hd, s);
+    MSA_REQUIRE(ok, MSA_ERR_HIP, "msa_paged_attention: the kernel's LDS was refused");
+    MSA_CHECK_LAUNCH("msa_paged_attention (tiles)");
   }
-  MSA_CHECK_LAUNCH("msa_paged_attention");
-  if (p.splits > 1) {
-    hipLaunchKernelGGL(paged_combine_kernel, dim3((unsigned)b->M, (unsigned)a->heads), dim3(64), 0, s, k, c->hd);
+  if (p.row_tiles > 0) {
+    k.splits = p.splits;
+    k.row_blocks = p.row_blocks;
+    switch (format) {
+      case PG_F16: msa_launch_paged_rows_f16(k, c->hd, p.row_tiles, s); break;
+      case PG_BF16: msa_launch_paged_rows_bf16(k, c->hd, p.row_tiles, s); break;
+      case PG_E4M3: msa_launch_paged_rows_e4m3(k, c->hd, p.row_tiles, s); break;
+      default: msa_launch_paged_rows_i8(k, c->hd, p.row_tiles, s); break;
+    }
+    MSA_CHECK_LAUNCH("msa_paged_attention (rows)");
+  }
+  if (p.splits > 1 || p.tile_splits > 1) {
+    hipLaunchKernelGGL(paged_combine_kernel, dim3((unsigned)b->M, (unsigned)a->heads), dim3(64), 0, s, k, c->hd,
+                       p.row_tiles > 0 ? p.splits : 1, p.tile_blocks > 0 ? p.tile_splits : 1);
     MSA_CHECK_LAUNCH("msa_paged_attention (splits)");
   }
   return MSA_OK;

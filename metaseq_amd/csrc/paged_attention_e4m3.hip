@@ -1,6 +1,10 @@
-// Attention over pages, few rows per sequence, e4m3 pages
+// Attention over pages: e4m3 pages
 #include "paged_attention.h"
 
 void msa_launch_paged_rows_e4m3(const PagedAttention& a, int hd, int row_tiles, hipStream_t stream) {
   pa_launch_rows_of<PG_E4M3>(a, hd, row_tiles, stream);
+}
+
+bool msa_launch_paged_tiles_e4m3(const PagedAttention& a, int hd, hipStream_t stream) {
+  return pa_launch_tiles_of<PG_E4M3>(a, hd, stream);
 }

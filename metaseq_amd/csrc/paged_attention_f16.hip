@@ -1,6 +1,10 @@
-// Attention over pages, few rows per sequence, fp16 pages
+// Attention over pages: fp16 pages
 #include "paged_attention.h"
 
 void msa_launch_paged_rows_f16(const PagedAttention& a, int hd, int row_tiles, hipStream_t stream) {
   pa_launch_rows_of<PG_F16>(a, hd, row_tiles, stream);
+}
+
+bool msa_launch_paged_tiles_f16(const PagedAttention& a, int hd, hipStream_t stream) {
+  return pa_launch_tiles_of<PG_F16>(a, hd, stream);
 }
