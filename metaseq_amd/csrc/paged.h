@@ -29,6 +29,7 @@ struct PagedAttention {
   float scale;
 };
 
+typedef __attribute__((address_space(4))) int32_t pg_uniform_i32;
 typedef uint32_t pg_u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t pg_u4 __attribute__((ext_vector_type(4)));
 

@@ -133,6 +133,15 @@ __device__ __forceinline__ float pa_quads_sum(float v) {
   return v + __shfl_xor(v, 32, MSA_WAVE);
 }
 
+// Of the N keys from `key` on (N <= 16), as bits, those that some row at a position between lo and hi sees (of
+// consecutive tokens; lo == hi: that the row sees).
+template <int N>
+__device__ __forceinline__ uint32_t pa_seen(int key, int lo, int hi, int window, int sinks) {
+  auto upto = [&](int last) { return (1u << min(max(last - key + 1, 0), N)) - 1; };  // keys <= last
+  const uint32_t past = upto(hi);
+  return window > 0 ? past & (~upto(lo - window) | upto(sinks - 1)) : past;
+}
+
 // The tiles of KT keys that rows at positions lo .. hi see: those of the first `sinks` positions, then from the window's
 // start on.
 template <int KT>
@@ -165,9 +174,9 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
   const int s = blockIdx.x / a.row_blocks, rb = blockIdx.x - s * a.row_blocks;
   const int h = blockIdx.y, split = blockIdx.z;
   const int group = a.heads / a.kv_heads;
-  const int row0 = a.seq_start[s], pos = a.seq_pos[s];
-  int count = min(a.seq_start[s + 1], a.M) - row0;
-  count = min(count, a.max_count);
+  const pg_uniform_i32* seq_start = (const pg_uniform_i32*)(uintptr_t)a.seq_start;
+  const int row0 = seq_start[s], pos = ((const pg_uniform_i32*)(uintptr_t)a.seq_pos)[s];
+  const int count = min(min(seq_start[s + 1], a.M) - row0, a.max_count);
   if (pos < 0 || row0 < 0 || count <= 0 || count * group > a.few || rb * 16 * RT >= count * group) return;
   const int page = 1 << a.page_log2, rows = count * group, rho0 = rb * 16 * RT;
   const int limit = a.blocks * page - 1;  // last position that can be anywhere
@@ -493,12 +502,28 @@ __device__ __forceinline__ int pt_chunk_at(int p, int row) {  // the chunk that 
   return c < 0 ? c + CH : c;
 }
 
+// a pointer that is the same in all lanes, in scalar registers
+__device__ __forceinline__ const char* pt_uniform(const char* p) {
+  const uint64_t w = (uint64_t)p;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)w), hi = __builtin_amdgcn_readfirstlane((uint32_t)(w >> 32));
+  return (const char*)((uint64_t)hi << 32 | lo);
+}
+
 template <int F>
 __device__ __forceinline__ float16_t pt_mfma(pg_u4 a, pg_u4 b, float16_t c) {
   if (F == PG_BF16)
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
 }
+
+// pages of a tile's four groups of sixteen keys, -1: none
+struct PtPages {
+  int a, b, c, d;
+  __device__ __forceinline__ int of(int g16) const {
+    const int w = a, x = b, y = c, z = d;
+    return g16 < 2 ? (g16 < 1 ? w : x) : (g16 < 3 ? y : z);
+  }
+};
 
 template <int F, int HD>
 __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kernel(PagedAttention a) {
@@ -508,7 +533,6 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
   constexpr int KSTEPS = HD / 16, DBLK = (HD + 31) / 32;
   constexpr int CH = HD / 8;                    // 16-byte chunks of a key row in LDS, which holds 16-bit elements
   constexpr int ROWB = HD * 2, TILEB = PT_BN * ROWB;
-  constexpr int NI = TILEB / 1024;              // direct load instructions of a tile
   constexpr float SHIFT = X::SHIFT;
   extern __shared__ __attribute__((aligned(16))) char lds[];  // K, K, V, V
 
@@ -529,8 +553,9 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
   const int split = rest % a.splits, rb = a.row_blocks - 1 - rest / a.splits;
   const int s = unit_id / a.kv_heads, h = unit_id - s * a.kv_heads;
   if (s >= a.nseq) return;
-  const int row0 = a.seq_start[s], pos = a.seq_pos[s];
-  const int count = min(min(a.seq_start[s + 1], a.M) - row0, a.max_count);
+  const pg_uniform_i32* seq_start = (const pg_uniform_i32*)(uintptr_t)a.seq_start;
+  const int row0 = seq_start[s], pos = ((const pg_uniform_i32*)(uintptr_t)a.seq_pos)[s];
+  const int count = min(min(seq_start[s + 1], a.M) - row0, a.max_count);
   if (pos < 0 || row0 < 0 || count <= 0 || count * group <= a.few || rb * PT_BM >= count * group) return;
   const int page = 1 << a.page_log2, rows = count * group, rho0 = rb * PT_BM;
   const int limit = a.blocks * page - 1;
@@ -575,60 +600,70 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
     }
   }
 
-  // ---- tiles ----
-  const int32_t* table = a.table + (int64_t)s * a.table_stride;
+  // ---- tiles.  (The table is read through the scalar cache: a vector load would be waited for together with all the
+  // loads to LDS in front of it) ----
+  const pg_uniform_i32* table = (const pg_uniform_i32*)(uintptr_t)(a.table + (int64_t)s * a.table_stride);
   // page of the sixteen keys g16 of tile i, -1 where there is none
   auto look = [&](int i, int g16) {
     const int block = (tiles.tile(i) * PT_BN + g16 * 16) >> a.page_log2;
-    const int pg = block < a.blocks ? table[block] : -1;
-    return pg >= 0 && pg < a.pages ? pg : -1;
+    const int pg = table[min(block, a.blocks - 1)];
+    return block < a.blocks && (unsigned)pg < (unsigned)a.pages ? pg : -1;
   };
   const int64_t unit = (int64_t)page * HD * ES;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(pt_lds_void*)lds;
-  // 16 bits: instruction u of the tile (every fourth is this wave's) fills 64 consecutive places
-  auto issue = [&](int i, int slot, const int (&pg)[4]) {
-    const int key0 = tiles.tile(i) * PT_BN;
+  // 16 bits.  Keys: the sixteen of this wave, which are of one page, fill its sixteen rows of the tile.  Values: every
+  // fourth group of eight rows (dimensions) is this wave's; a lane has the same chunk (eight keys) in all of them.
+  constexpr int KI = (16 * CH + 63) / 64, VI = (HD / 8 + 3) / 4;
+  uint32_t koff[B8 ? 1 : KI];
+  const int vrow = wave * 8 + (lane >> 3), vc = pt_chunk_at<8>(lane & 7, vrow);
+  if (!B8) {
 #pragma unroll
-    for (int u = 0; u < (NI + 3) / 4; ++u) {
-      const int n = u * 4 + wave;
-      if (NI % 4 != 0 && n >= NI) break;
-      {
-        const int at = n * 64 + lane, row = at / CH, c = pt_chunk_at<CH>(at % CH, row);
-        const int p = row < 32 ? (row < 16 ? pg[0] : pg[1]) : (row < 48 ? pg[2] : pg[3]);
-        const char* from = (const char*)a.k_pages + ((int64_t)max(p, 0) * a.kv_heads + h) * unit +
-                           (int64_t)((key0 + row) & (page - 1)) * ROWB + c * 16;
-        const uint32_t la = lds0 + slot * TILEB + n * 1024;
-        asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(la) : "memory");
+    for (int u = 0; u < KI; ++u) {
+      const int at = u * 64 + lane, row = min(at / CH, 15);
+      koff[u] = row * ROWB + pt_chunk_at<CH>(at % CH, row) * 16;
+    }
+  }
+  auto issue = [&](int i, int slot, PtPages pg) {
+    const int key0 = tiles.tile(i) * PT_BN, in = page - 1;
+    {
+      const int p = pg.of(wave);
+      const char* from = (const char*)a.k_pages + ((int64_t)max(p, 0) * a.kv_heads + h) * unit + (int64_t)((key0 + wave * 16) & in) * ROWB;
+#pragma unroll
+      for (int u = 0; u < KI; ++u) {
+        const uint32_t la = lds0 + slot * TILEB + wave * 16 * ROWB + u * 1024;
+        if ((u + 1) * 64 <= 16 * CH || lane < 16 * CH - u * 64)
+          asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(koff[u]), "s"(pt_uniform(from)), "s"(la) : "memory");
       }
-      {
-        const int at = n * 64 + lane, row = at / 8, c = pt_chunk_at<8>(at % 8, row), key = key0 + c * 8;
-        const int p = c < 4 ? (c < 2 ? pg[0] : pg[1]) : (c < 6 ? pg[2] : pg[3]);
-        const char* from = (const char*)a.v_pages + ((int64_t)max(p, 0) * a.kv_heads + h) * unit +
-                           ((int64_t)row * page + (key & (page - 1))) * 2;
-        const uint32_t la = lds0 + (2 + slot) * TILEB + n * 1024;
+    }
+    auto at = [&](int k) { return ((int64_t)max(pg.of(k), 0) * a.kv_heads + h) * unit + ((key0 + k * 16) & in) * 2; };
+    const int64_t at0 = at(0), at1 = at(1), at2 = at(2), at3 = at(3);
+    const char* from = (const char*)a.v_pages + (vc < 4 ? (vc < 2 ? at0 : at1) : (vc < 6 ? at2 : at3)) + (vc & 1) * 16 + vrow * page * 2;
+#pragma unroll
+    for (int u = 0; u < VI; ++u) {
+      const uint32_t la = lds0 + (2 + slot) * TILEB + (u * 4 + wave) * 1024;
+      if (HD % 32 == 0 || u * 4 + wave < HD / 8)
         asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(la) : "memory");
-      }
+      from += page * 64;
     }
   };
   // whether any row of the workgroup sees the key
   const int g_lo = position(rho0), g_hi = position(rho0 + PT_BM - 1);
-  auto anyone = [&](int key) { return key <= g_hi && (a.window <= 0 || key > g_lo - a.window || key < a.sinks); };
+  auto anyone = [&](int key) { return pa_seen<1>(key, g_lo, g_hi, a.window, a.sinks) != 0; };
   // 8 bits: chunks of 16 elements, registers in between
   constexpr int CB = HD / 16, KN = (PT_BN * CB + PT_THREADS - 1) / PT_THREADS, VN = (HD * 4 + PT_THREADS - 1) / PT_THREADS;
   pg_u4 kr[B8 ? KN : 1], vr[B8 ? VN : 1], vx;
   int kx[B8 ? KN : 1], ke = 0, ve = 0;  // the rows' exponents; those of key `lane` of the tile
   const int vg = threadIdx.x & 3;       // the sixteen keys that the thread's chunks of V belong to
-  auto fetch = [&](int i, const int (&pg)[4]) {
+  auto fetch = [&](int i, PtPages pg) {
     const int key0 = tiles.tile(i) * PT_BN;
-    auto page_of = [&](int g16) { return g16 < 2 ? (g16 < 1 ? pg[0] : pg[1]) : (g16 < 3 ? pg[2] : pg[3]); };
 #pragma unroll
     for (int j = 0; j < KN; ++j) {
       const int at = min((int)threadIdx.x + j * PT_THREADS, PT_BN * CB - 1), row = at / CB, c = at % CB;
-      const int64_t up = ((int64_t)max(page_of(row >> 4), 0) * a.kv_heads + h) * page + ((key0 + row) & (page - 1));
+      const int64_t up = ((int64_t)max(pg.of(row >> 4), 0) * a.kv_heads + h) * page + ((key0 + row) & (page - 1));
       kr[j] = *(const pg_u4*)((const char*)a.k_pages + up * HD + c * 16);
       kx[j] = a.k_exp[up];
     }
-    const int64_t uv = (int64_t)max(page_of(vg), 0) * a.kv_heads + h;
+    const int64_t uv = (int64_t)max(pg.of(vg), 0) * a.kv_heads + h;
     const int in = (key0 + vg * 16) & (page - 1);
 #pragma unroll
     for (int j = 0; j < VN; ++j) {
@@ -636,16 +671,15 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
       vr[j] = *(const pg_u4*)((const char*)a.v_pages + uv * unit + (int64_t)row * page + in);
     }
     vx = *(const pg_u4*)(a.v_exp + uv * page + in);
-    const int64_t ul = ((int64_t)max(page_of(lane >> 4), 0) * a.kv_heads + h) * page + ((key0 + lane) & (page - 1));
+    const int64_t ul = ((int64_t)max(pg.of(lane >> 4), 0) * a.kv_heads + h) * page + ((key0 + lane) & (page - 1));
     ke = a.k_exp[ul];
     ve = a.v_exp[ul];
   };
   auto wave_most = [](int v) { return (int)wave_max((float)v); };
   // (returns the exponents that the tile's keys and values are relative to)
-  auto stage = [&](int i, int slot, const int (&pg)[4], int& ek, int& ev) {
+  auto stage = [&](int i, int slot, PtPages pg, int& ek, int& ev) {
     const int key0 = tiles.tile(i) * PT_BN;
-    auto page_of = [&](int g16) { return g16 < 2 ? (g16 < 1 ? pg[0] : pg[1]) : (g16 < 3 ? pg[2] : pg[3]); };
-    const bool mine = page_of(lane >> 4) >= 0 && anyone(key0 + lane);
+    const bool mine = pg.of(lane >> 4) >= 0 && anyone(key0 + lane);
     ek = __builtin_amdgcn_readfirstlane(wave_most(mine ? ke : -127));
     ev = max(ev, __builtin_amdgcn_readfirstlane(wave_most(mine ? ve : -127)));
     char* kt = lds + slot * TILEB;
@@ -665,19 +699,18 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
       }
     }
     half8_t f[2];
-    pg_u4 keep;
-    const bool there = page_of(vg) >= 0;
+    const uint32_t seen = pg.of(vg) >= 0 ? pa_seen<16>(key0 + vg * 16, g_lo, g_hi, a.window, a.sinks) : 0;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const bool sees = there && anyone(key0 + vg * 16 + k);
-      f[k >> 3][k & 7] = (half_t)(sees ? power((int)(int8_t)(vx[k >> 2] >> ((k & 3) * 8)) - ev) : 0.f);
-      keep[k >> 2] = ((k & 3) ? keep[k >> 2] : 0) | (sees ? 0xffu << ((k & 3) * 8) : 0);
-    }
+    for (int k = 0; k < 16; ++k) f[k >> 3][k & 7] = (half_t)power((int)(int8_t)(vx[k >> 2] >> ((k & 3) * 8)) - ev);
 #pragma unroll
     for (int j = 0; j < VN; ++j) {
       const int at = threadIdx.x + j * PT_THREADS, row = at >> 2;
       if ((HD * 4) % PT_THREADS == 0 || at < HD * 4) {
-        const pg_u4 w = vr[j] & keep;
+        pg_u4 w = vr[j];
+        if (seen != 0xffff) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = pa_keep<F>(w[k], seen >> (4 * k));
+        }
 #pragma unroll
         for (int e = 0; e < 2; ++e)
           *(half8_t*)(vt + row * 128 + pt_place<8>(2 * vg + e, row) * 16) = __builtin_bit_cast(half8_t, pa_operand<F>(w, e)) * f[e];
@@ -688,88 +721,105 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
   // ---- fragments: K block ib, step ks: row with bits 2 and 3 of n32 exchanged, chunk 2 ks + hl.  V^T block db, step c (16
   // keys): row 32 db + n32, chunk 2 c + hl ----
   const int krow = (n32 & ~12) | ((n32 & 4) << 1) | ((n32 & 8) >> 1);
+  auto v_at = [&](const char* vt, int db, int st) {
+    const int row = HD % 32 == 0 ? db * 32 + n32 : min(db * 32 + n32, HD - 1);
+    return *(const pg_u4*)(vt + row * 128 + pt_place<8>(2 * st + hl, row) * 16);
+  };
+  constexpr int G = F == PG_BF16 ? PG_BF16 : PG_F16;  // LDS holds 16 bits in every format
+  const float16_t zero16 = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   float16_t o[DBLK];
 #pragma unroll
-  for (int d = 0; d < DBLK; ++d)
-#pragma unroll
-    for (int v = 0; v < 16; ++v) o[d][v] = 0.f;
+  for (int d = 0; d < DBLK; ++d) o[d] = zero16;
   float m = -INFINITY, l = 0.f;
-  int E = -127, ek[2] = {0, 0}, ev[2] = {-127, -127};
-  int pg[2][4];  // pages of the tile at hand and the next one's
-  auto look4 = [&](int i, int (&p)[4]) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) p[k] = look(min(i, it_end - 1), k);
+  int E = -127, ek = 0, ev = -127;  // what the accumulators are relative to, and this tile's keys and values
+  auto look4 = [&](int i) {
+    const int j = min(i, it_end - 1);
+    return PtPages{look(j, 0), look(j, 1), look(j, 2), look(j, 3)};
   };
+  PtPages pg = {-1, -1, -1, -1}, next = pg;  // this tile's and the next one's
   if (it0 < it_end) {
-    look4(it0, pg[0]);
-    look4(it0 + 1, pg[1]);
+    pg = look4(it0);
+    next = look4(it0 + 1);
     if (B8) {
-      fetch(it0, pg[0]);
-      stage(it0, 0, pg[0], ek[0], ev[0]);
+      fetch(it0, pg);
+      stage(it0, 0, pg, ek, ev);
     } else {
-      issue(it0, 0, pg[0]);
+      issue(it0, 0, pg);
     }
   }
   for (int i = it0; i < it_end; ++i) {
     const int slot = (i - it0) & 1;
-    const int here = (pg[0][0] >= 0 ? 1 : 0) | (pg[0][1] >= 0 ? 2 : 0) | (pg[0][2] >= 0 ? 4 : 0) | (pg[0][3] >= 0 ? 8 : 0);
+    const int here = (pg.a >= 0 ? 1 : 0) | (pg.b >= 0 ? 2 : 0) | (pg.c >= 0 ? 4 : 0) | (pg.d >= 0 ? 8 : 0);
     if (!B8) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();  // the tile is complete, and the other slots are free
     if (i + 1 < it_end) {
-      if (B8) fetch(i + 1, pg[1]);
-      else issue(i + 1, slot ^ 1, pg[1]);
+      if (B8) fetch(i + 1, next);
+      else issue(i + 1, slot ^ 1, next);
     }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) pg[0][k] = pg[1][k];
-    if (i + 2 < it_end) look4(i + 2, pg[1]);
+    pg = next;
+    next = look4(i + 2);
 
     const char* kt = lds + slot * TILEB;
-    const char* vt = lds + (2 + slot) * TILEB;
+    char* vt = lds + (2 + slot) * TILEB;
     const int key0 = tiles.tile(i) * PT_BN;
     const bool whole = key0 + PT_BN - 1 <= p_lo && (a.window <= 0 || key0 > p_hi - a.window || key0 + PT_BN <= a.sinks) && here == 15;
+    // Tiles of which not every row sees every key (of the workgroup): values of keys that no row sees may be anything and
+    // become zeros.  Whether there is one then that is not finite: it must reach the rows that see it only (0 times
+    // infinity is NaN), so it is added to those and left out of the product.
+    bool odd = false;
+    if (F != PG_I8 && !(key0 + PT_BN - 1 <= g_lo && (a.window <= 0 || key0 > g_hi - a.window || key0 + PT_BN <= a.sinks) && here == 15)) {
+#pragma unroll 1
+      for (int at = threadIdx.x; at < HD * 8; at += PT_THREADS) {
+        const int key = key0 + pt_chunk_at<8>(at & 7, at >> 3) * 8;
+        const bool there = (here >> ((key - key0) >> 4)) & 1;
+        const uint32_t seen = there ? pa_seen<8>(key, g_lo, g_hi, a.window, a.sinks) : 0;
+        pg_u4 v = *(pg_u4*)(vt + at * 16);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          v[k] = pa_keep<G>(v[k], seen >> (2 * k));
+          odd |= pa_not_finite<G>(v[k], 0) != 0;
+        }
+        if (seen != 255) *(pg_u4*)(vt + at * 16) = v;
+      }
+      odd = __syncthreads_or(odd);
+    }
     // (a wave whose rows see nothing of the tile has nothing to do)
     const bool none = key0 > p_hi || w0 >= rows || (a.window > 0 && key0 + PT_BN - 1 <= p_lo - a.window && key0 >= a.sinks);
-    if (!none) {
+    const float c = B8 ? ldexpf(qs, ek) : qs;
+    // Two copies: tiles that every row of the wave sees whole, and others.
+    auto attend = [&](auto edge) {
+      constexpr bool EDGE = decltype(edge)::value;
       float16_t sc[2];
-#pragma unroll
-      for (int ib = 0; ib < 2; ++ib)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) sc[ib][v] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < KSTEPS; ++ks)
 #pragma unroll
         for (int ib = 0; ib < 2; ++ib) {
           const int row = ib * 32 + krow;
           const pg_u4 k = *(const pg_u4*)(kt + row * ROWB + pt_place<CH>(2 * ks + hl, row) * 16);
-          sc[ib] = pt_mfma<F>(k, qf[ks], sc[ib]);
+          sc[ib] = pt_mfma<F>(k, qf[ks], ks == 0 ? zero16 : sc[ib]);
         }
-      const float c = B8 ? ldexpf(qs, ek[slot]) : qs;
-      // key of element v of block ib
-      auto key_of = [&](int ib, int v) { return key0 + ib * 32 + (v >> 3) * 16 + hl * 8 + (v & 7); };
-      float top = -INFINITY;
-      if (whole) {
+      float z[32];  // keys key0 + 16 (j / 8) + 8 hl + j % 8
 #pragma unroll
-        for (int ib = 0; ib < 2; ++ib)
+      for (int j = 0; j < 32; ++j) z[j] = sc[j >> 4][j & 15];
+      uint32_t sees = ~0u;  // of those keys, the row's
+      if (EDGE) {
+        sees = 0;
 #pragma unroll
-          for (int v = 0; v < 16; ++v) top = fmaxf(top, sc[ib][v]);
-      } else {
+        for (int g8 = 0; g8 < 4; ++g8)
+          sees |= pa_seen<8>(key0 + g8 * 16 + hl * 8, pn, pn, a.window, a.sinks) * ((here >> g8) & 1) << (g8 * 8);
 #pragma unroll
-        for (int ib = 0; ib < 2; ++ib)
-#pragma unroll
-          for (int v = 0; v < 16; ++v) {
-            const int key = key_of(ib, v);
-            if (!(here >> (ib * 2 + (v >> 3)) & 1) || key > pn || (a.window > 0 && key <= pn - a.window && key >= a.sinks))
-              sc[ib][v] = -INFINITY;
-            top = fmaxf(top, sc[ib][v]);
-          }
+        for (int j = 0; j < 32; ++j) z[j] = (sees >> j) & 1 ? z[j] : -INFINITY;
       }
+      float top = z[0];
+#pragma unroll
+      for (int j = 1; j < 32; ++j) top = fmaxf(top, z[j]);
       top *= c;
-      if (B8 && ev[slot] > E) {
+      if (B8 && ev > E) {
 #pragma unroll
         for (int d = 0; d < DBLK; ++d)
 #pragma unroll
-          for (int v = 0; v < 16; ++v) o[d][v] = ldexpf(o[d][v], E - ev[slot]);
-        E = ev[slot];
+          for (int v = 0; v < 16; ++v) o[d][v] = ldexpf(o[d][v], E - ev);
+        E = ev;
       }
       if (__ballot(top > m + PA_LAZY)) {
         const float to = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, MSA_WAVE)));
@@ -782,88 +832,65 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
           for (int v = 0; v < 16; ++v) o[d][v] *= w;
       }
       const float off = (m == -INFINITY ? 0.f : m) - SHIFT;
-      pg_u4 p[4];  // step 2 ib + c of the product with V
+      pg_u4 p[4];  // steps of sixteen keys of the product with V
       float sum[2] = {0.f, 0.f};
 #pragma unroll
-      for (int ib = 0; ib < 2; ++ib)
+      for (int st = 0; st < 4; ++st) {
+        float e[8];
 #pragma unroll
-        for (int cc = 0; cc < 2; ++cc) {
-          float e[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[ib][cc * 8 + j], c, -off));
-            sum[j & 1] += e[j];
-          }
-          if (F == PG_BF16) {
-            bf16x8_t w;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) w[j] = (bf16_t)e[j];
-            p[ib * 2 + cc] = __builtin_bit_cast(pg_u4, w);
-          } else {
-            half8_t w;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) w[j] = (half_t)e[j];
-            p[ib * 2 + cc] = __builtin_bit_cast(pg_u4, w);
-          }
+        for (int j = 0; j < 8; ++j) {
+          e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[st * 8 + j], c, -off));
+          sum[j & 1] += e[j];
         }
+        if (F == PG_BF16) {
+          bf16x8_t w;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w[j] = (bf16_t)e[j];
+          p[st] = __builtin_bit_cast(pg_u4, w);
+        } else {
+          half8_t w;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w[j] = (half_t)e[j];
+          p[st] = __builtin_bit_cast(pg_u4, w);
+        }
+      }
       l += sum[0] + sum[1];
-      auto v_at = [&](int db, int st) {
-        const int row = HD % 32 == 0 ? db * 32 + n32 : min(db * 32 + n32, HD - 1);
-        return *(const pg_u4*)(vt + row * 128 + pt_place<8>(2 * st + hl, row) * 16);
-      };
-      if (whole) {
-#pragma unroll
-        for (int st = 0; st < 4; ++st)
-#pragma unroll
-          for (int db = 0; db < DBLK; ++db) o[db] = pt_mfma<F>(v_at(db, st), p[st], o[db]);
-      } else {
-        // as in the kernel above: values that no row sees are zeros, and those that are not finite reach the rows that
-        // see them only
-#pragma unroll
-        for (int st = 0; st < 4; ++st) {
-          uint32_t seen = 0;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int key = key0 + st * 16 + hl * 8 + j;
-            const bool sees = (here >> st & 1) && key <= p_hi && (a.window <= 0 || key > p_lo - a.window || key < a.sinks);
-            seen |= sees ? 1u << j : 0;
-          }
-#pragma unroll
-          for (int db = 0; db < DBLK; ++db) {
-            constexpr int G = F == PG_BF16 ? PG_BF16 : PG_F16;  // LDS holds 16 bits in every format
-            pg_u4 v = v_at(db, st);
-            bool odd = false;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              v[k] = pa_keep<G>(v[k], seen >> (2 * k));
-              odd |= pa_not_finite<G>(v[k], 0) != 0;
-            }
-            if (__ballot(odd)) {
+      if (EDGE && F != PG_I8) {
+        if (odd) {  // (an infinity or a NaN times a probability is itself)
 #pragma unroll 1
-              for (int kind = 1; kind <= 3; ++kind) {
-                pg_u4 ones;
+          for (int j = 0; j < PT_BN; ++j) {
+            int hl4 = hl * 4;  // (formed anew: 64 addresses would be kept through both loops)
+            asm volatile("" : "+v"(hl4));
+            const bool mine = (pa_seen<1>(key0 + j, pn, pn, a.window, a.sinks) & (here >> (j >> 4))) != 0;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) ones[k] = pa_not_finite<G>(v[k], kind);
-                float16_t hit;
+            for (int db = 0; db < DBLK; ++db)
 #pragma unroll
-                for (int k = 0; k < 16; ++k) hit[k] = 0.f;
-                hit = pt_mfma<F>(ones, p[st], hit);
-#pragma unroll
-                for (int k = 0; k < 16; ++k)
-                  if (hit[k] != 0.f) o[db][k] += kind == 1 ? INFINITY : kind == 2 ? -INFINITY : NAN;
+              for (int v = 0; v < 16; ++v) {
+                const int row = min(db * 32 + (v >> 2) * 8 + hl4 + (v & 3), HD - 1);
+                const uint32_t x = *(const uint16_t*)(vt + row * 128 + pt_place<8>(j >> 3, row) * 16 + (j & 7) * 2);
+                const float f = G == PG_BF16 ? __builtin_bit_cast(float, x << 16) : (float)__builtin_bit_cast(half_t, (uint16_t)x);
+                o[db][v] += (mine & !(fabsf(f) < INFINITY)) ? f : 0.f;
               }
-#pragma unroll
-              for (int k = 0; k < 4; ++k) v[k] = pa_finite<G>(v[k]);
-            }
-            o[db] = pt_mfma<F>(v, p[st], o[db]);
           }
         }
       }
-    }
-    if (B8 && i + 1 < it_end) {
-      ev[slot ^ 1] = ev[slot];
-      stage(i + 1, slot ^ 1, pg[0], ek[slot ^ 1], ev[slot ^ 1]);
-    }
+#pragma unroll
+      for (int st = 0; st < 4; ++st)
+#pragma unroll
+        for (int db = 0; db < DBLK; ++db) {
+          pg_u4 v = v_at(vt, db, st);
+          if (EDGE && F != PG_I8) {
+            if (odd) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) v[k] = pa_finite<G>(v[k]);
+            }
+          }
+          o[db] = pt_mfma<F>(v, p[st], o[db]);
+        }
+    };
+    if (whole) attend(std::false_type{});
+    else if (!none) attend(std::true_type{});
+    if (B8 && i + 1 < it_end) stage(i + 1, slot ^ 1, pg, ek, ev);
   }
 
   // ---- O^T: row n32, dimensions 32 db + 8 blk + 4 hl + r ----

@@ -161,6 +161,241 @@ __global__ __launch_bounds__(256) void read_rows_kernel(PagedRows a) {
   }
 }
 
+// Workgroup = 64 consecutive positions (from a multiple of 64 on) of a sequence, one key/value head: the form for portions of
+// prompts.  Rows are read and written 16 bytes a lane; values cross over in LDS, and leave (or come) as 16 bytes of one
+// dimension's consecutive positions.  Bound by HBM.
+constexpr int PB = 64;  // positions of a block
+constexpr int BLOCK_TOKENS = 8;
+
+struct Block {
+  int first, begin, end, row;  // positions that are new: begin .. end - 1; the row of position `first`
+};
+__device__ __forceinline__ bool block_of(const PagedRows& a, int s, int i, Block& b) {
+  const pg_uniform_i32* start = (const pg_uniform_i32*)(uintptr_t)a.b.seq_start;
+  const int row0 = start[s], pos = ((const pg_uniform_i32*)(uintptr_t)a.b.seq_pos)[s];
+  const int64_t count = min(min(start[s + 1], a.b.M) - row0, a.b.max_count);
+  const int64_t first = ((int64_t)(pos >> 6) + i) * PB;
+  if (pos < 0 || row0 < 0 || count <= 0 || first >= pos + count || pos + count > INT32_MAX) return false;
+  b.first = (int)first;
+  b.begin = max(pos, b.first);
+  b.end = (int)min(pos + count, first + PB);
+  b.row = row0 + b.first - pos;
+  return true;
+}
+
+// lanes that share a row of HD elements, 8 each: a power of two
+template <int HD>
+constexpr int row_lanes() { return HD <= 64 ? 8 : HD <= 128 ? 16 : 32; }
+
+template <int DT, int F, int HD>
+__global__ __launch_bounds__(256) void append_block_kernel(PagedRows a, int blocks) {
+  typedef typename Elem<DT>::T T;
+  constexpr int ES = F < PG_E4M3 ? 2 : 1, LR = row_lanes<HD>(), RP = 256 / LR, N = PB / RP;
+  constexpr int STRIDE = HD * ES + 4;                  // of an LDS row: columns are read without bank conflicts
+  constexpr int G = 16 / ES, NG = PB / G;              // positions of 16 bytes of a dimension
+  __shared__ __attribute__((aligned(16))) char lds[PB * STRIDE];
+  const int s = blockIdx.x / blocks, h = blockIdx.y, lane = threadIdx.x % LR, r0 = threadIdx.x / LR;
+  Block b;
+  if (!block_of(a, s, blockIdx.x - s * blocks, b)) return;
+  const int page = 1 << a.page_log2;
+  pg_u4 k[N], v[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int p = b.first + r0 + i * RP;
+    k[i] = v[i] = pg_u4{0, 0, 0, 0};
+    if (p >= b.begin && p < b.end && lane * 8 < HD) {
+      const int64_t row = b.row + r0 + i * RP;
+      k[i] = *(const pg_u4*)((const T*)a.k + row * a.ldk + h * HD + lane * 8);
+      v[i] = *(const pg_u4*)((const T*)a.v + row * a.ldv + h * HD + lane * 8);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int p = b.first + r0 + i * RP, at = r0 + i * RP;
+    const bool here = p >= b.begin && p < b.end;
+    const int pg = here ? page_of(a, s, p) : -1;
+    const int64_t unit = (int64_t)pg * a.c.kv_heads + h, place = unit * page + (p & (page - 1));
+    if (ES == 2) {
+      if (pg >= 0 && lane * 8 < HD) *(pg_u4*)((T*)a.c.k_pages + place * HD + lane * 8) = k[i];
+      if (lane * 8 < HD) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *(uint32_t*)(lds + at * STRIDE + lane * 16 + j * 4) = v[i][j];
+      }
+      continue;
+    }
+    const float cap = largest<DT, F>();
+    float kx[8], vx[8], km = 0.f, vm = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      kx[j] = (float)__builtin_bit_cast(T, (uint16_t)(k[i][j >> 1] >> ((j & 1) * 16)));
+      vx[j] = (float)__builtin_bit_cast(T, (uint16_t)(v[i][j >> 1] >> ((j & 1) * 16)));
+      km = fmaxf(km, magnitude(kx[j]));
+      vm = fmaxf(vm, magnitude(vx[j]));
+    }
+#pragma unroll
+    for (int o = LR / 2; o > 0; o >>= 1) {
+      km = fmaxf(km, __shfl_xor(km, o, MSA_WAVE));
+      vm = fmaxf(vm, __shfl_xor(vm, o, MSA_WAVE));
+    }
+    const int ke = exponent_of<F>(fminf(km, cap)), ve = exponent_of<F>(fminf(vm, cap));
+    const float ks = inverse_power(ke), vs = inverse_power(ve);
+    auto held = [&](float x) { return x > cap ? cap : x < -cap ? -cap : x; };
+    auto four = [&](const float* x, float f) {
+      return code2<F>(held(x[0]) * f, held(x[1]) * f) | code2<F>(held(x[2]) * f, held(x[3]) * f) << 16;
+    };
+    if (lane * 8 < HD) {
+      if (pg >= 0) *(pg_u2*)((uint8_t*)a.c.k_pages + place * HD + lane * 8) = pg_u2{four(kx, ks), four(kx + 4, ks)};
+      *(uint32_t*)(lds + at * STRIDE + lane * 8) = four(vx, vs);
+      *(uint32_t*)(lds + at * STRIDE + lane * 8 + 4) = four(vx + 4, vs);
+    }
+    if (pg >= 0 && lane == 0) a.c.k_exp[place] = (int8_t)ke, a.c.v_exp[place] = (int8_t)ve;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < HD * NG; i += 256) {
+    const int d = i / NG, g = i % NG, p = b.first + g * G;
+    if (p + G <= b.begin || p >= b.end) continue;
+    const int pg = page_of(a, s, p);
+    if (pg < 0) continue;
+    char* to = (char*)a.c.v_pages + ((((int64_t)pg * a.c.kv_heads + h) * HD + d) * page + (p & (page - 1))) * ES;
+    const char* from = lds + g * G * STRIDE + d * ES;
+    if (p >= b.begin && p + G <= b.end) {
+      pg_u4 w;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (ES == 2) {
+          w[j] = *(const uint16_t*)(from + 2 * j * STRIDE) | (uint32_t)*(const uint16_t*)(from + (2 * j + 1) * STRIDE) << 16;
+        } else {
+          w[j] = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[j] |= (uint32_t)*(const uint8_t*)(from + (4 * j + e) * STRIDE) << (8 * e);
+        }
+      }
+      *(pg_u4*)to = w;
+    } else {  // positions beside the new ones stay as they are
+      for (int j = max(b.begin - p, 0); j < min(b.end - p, G); ++j) {
+        if (ES == 2) ((uint16_t*)to)[j] = *(const uint16_t*)(from + j * STRIDE);
+        else ((uint8_t*)to)[j] = *(const uint8_t*)(from + j * STRIDE);
+      }
+    }
+  }
+}
+
+template <int DT, int F, int HD>
+__global__ __launch_bounds__(256) void read_block_kernel(PagedRows a, int blocks) {
+  typedef typename Elem<DT>::T T;
+  constexpr int ES = F < PG_E4M3 ? 2 : 1, LR = row_lanes<HD>(), RP = 256 / LR, N = PB / RP;
+  constexpr int STRIDE = HD * ES + 4, G = 16 / ES, NG = PB / G, NV = (HD * NG + 255) / 256;
+  __shared__ __attribute__((aligned(16))) char lds[PB * STRIDE];
+  const int s = blockIdx.x / blocks, h = blockIdx.y, lane = threadIdx.x % LR, r0 = threadIdx.x / LR;
+  Block b;
+  if (!block_of(a, s, blockIdx.x - s * blocks, b)) return;
+  const int page = 1 << a.page_log2;
+  // 8 codes (or two words more of 16 bits) times 2^e as 16 bytes of T
+  auto rows_of = [](pg_u4 w, int e) {
+    if (ES == 2) return w;
+    pg_u4 out;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t two = w[j >> 1] >> ((j & 1) * 16);
+      const T x = (T)ldexpf(value_of<F>((uint8_t)two), e), y = (T)ldexpf(value_of<F>((uint8_t)(two >> 8)), e);
+      out[j] = (uint32_t)__builtin_bit_cast(uint16_t, x) | (uint32_t)__builtin_bit_cast(uint16_t, y) << 16;
+    }
+    return out;
+  };
+  pg_u4 v[NV], k[N];
+  int ke[N], ve[N];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int at = threadIdx.x + i * 256, d = at / NG, p = b.first + (at % NG) * G;
+    v[i] = pg_u4{0, 0, 0, 0};
+    const int pg = at < HD * NG && p + G > b.begin && p < b.end ? page_of(a, s, p) : -1;
+    if (pg >= 0) v[i] = *(const pg_u4*)((const char*)a.c.v_pages + ((((int64_t)pg * a.c.kv_heads + h) * HD + d) * page + (p & (page - 1))) * ES);
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int p = b.first + r0 + i * RP;
+    const int pg = p >= b.begin && p < b.end ? page_of(a, s, p) : -1;
+    const int64_t place = ((int64_t)pg * a.c.kv_heads + h) * page + (p & (page - 1));
+    k[i] = pg_u4{0, 0, 0, 0};
+    ke[i] = ve[i] = 0;
+    if (pg >= 0 && lane * 8 < HD) {
+      if (ES == 2) {
+        k[i] = *(const pg_u4*)((const T*)a.c.k_pages + place * HD + lane * 8);
+      } else {
+        const pg_u2 w = *(const pg_u2*)((const uint8_t*)a.c.k_pages + place * HD + lane * 8);
+        k[i][0] = w[0], k[i][1] = w[1];
+        ke[i] = a.c.k_exp[place], ve[i] = a.c.v_exp[place];
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int at = threadIdx.x + i * 256;
+    if (at >= HD * NG) break;
+    char* to = lds + (at % NG) * G * STRIDE + at / NG * ES;
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+      if (ES == 2) *(uint16_t*)(to + j * STRIDE) = (uint16_t)(v[i][j >> 1] >> ((j & 1) * 16));
+      else *(uint8_t*)(to + j * STRIDE) = (uint8_t)(v[i][j >> 2] >> ((j & 3) * 8));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int p = b.first + r0 + i * RP;
+    if (p >= b.begin && p < b.end && lane * 8 < HD)
+      *(pg_u4*)((T*)a.k_out + (int64_t)(b.row + r0 + i * RP) * a.ldk + h * HD + lane * 8) = rows_of(k[i], ke[i]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int p = b.first + r0 + i * RP;
+    if (p < b.begin || p >= b.end || lane * 8 >= HD) continue;
+    const char* from = lds + (r0 + i * RP) * STRIDE + lane * 8 * ES;
+    pg_u4 w = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 2 * ES; ++j) w[j] = *(const uint32_t*)(from + j * 4);
+    *(pg_u4*)((T*)a.v_out + (int64_t)(b.row + r0 + i * RP) * a.ldv + h * HD + lane * 8) = rows_of(w, ve[i]);
+  }
+}
+
+template <int DT, int F, int HD>
+void launch_rows_hd(const PagedRows& a, bool append, hipStream_t s) {
+  // (BLOCK_TOKENS: see below)
+  if (a.b.max_count < BLOCK_TOKENS) {
+    const dim3 grid((unsigned)a.b.M, (unsigned)((a.c.kv_heads + 3) / 4));
+    if (append) hipLaunchKernelGGL((append_rows_kernel<DT, F>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((read_rows_kernel<DT, F>), grid, dim3(256), 0, s, a);
+    return;
+  }
+  const int blocks = (a.b.max_count + PB - 2) / PB + 1;  // that max_count positions can meet
+  const dim3 grid((unsigned)(a.b.nseq * blocks), (unsigned)a.c.kv_heads);
+  if (append) hipLaunchKernelGGL((append_block_kernel<DT, F, HD>), grid, dim3(256), 0, s, a, blocks);
+  else hipLaunchKernelGGL((read_block_kernel<DT, F, HD>), grid, dim3(256), 0, s, a, blocks);
+}
+
+template <int DT, int F>
+void launch_rows_format(const PagedRows& a, bool append, hipStream_t s) {
+  switch (a.c.hd) {
+    case 64: return launch_rows_hd<DT, F, 64>(a, append, s);
+    case 80: return launch_rows_hd<DT, F, 80>(a, append, s);
+    case 96: return launch_rows_hd<DT, F, 96>(a, append, s);
+    case 128: return launch_rows_hd<DT, F, 128>(a, append, s);
+    case 192: return launch_rows_hd<DT, F, 192>(a, append, s);
+    default: return launch_rows_hd<DT, F, 256>(a, append, s);
+  }
+}
+
+void launch_rows(const PagedRows& a, bool append, hipStream_t s) {
+  if (a.c.dtype == MSA_F16) {
+    if (a.c.format == MSA_PAGES_SAME) return launch_rows_format<MSA_F16, PG_F16>(a, append, s);
+    if (a.c.format == MSA_PAGES_E4M3) return launch_rows_format<MSA_F16, PG_E4M3>(a, append, s);
+    return launch_rows_format<MSA_F16, PG_I8>(a, append, s);
+  }
+  if (a.c.format == MSA_PAGES_SAME) return launch_rows_format<MSA_BF16, PG_BF16>(a, append, s);
+  if (a.c.format == MSA_PAGES_E4M3) return launch_rows_format<MSA_BF16, PG_E4M3>(a, append, s);
+  return launch_rows_format<MSA_BF16, PG_I8>(a, append, s);
+}
+
 int check_rows(const msa_paged_cache* c, const msa_paged_batch* b, const void* k, int64_t ldk, const void* v, int64_t ldv,
                const char* who) {
   const int rc = msa_paged_check(c, b, who);
@@ -168,6 +403,7 @@ int check_rows(const msa_paged_cache* c, const msa_paged_batch* b, const void* k
   MSA_REQUIRE(k && v, MSA_ERR_INVALID_ARG, "%s: null pointer", who);
   MSA_REQUIRE(((uintptr_t)k | (uintptr_t)v) % 16 == 0, MSA_ERR_INVALID_ARG, "%s: keys and values must be 16-byte aligned", who);
   const int64_t n = (int64_t)c->kv_heads * c->hd;
+  MSA_REQUIRE((int64_t)b->nseq * ((b->max_count + 62) / 64 + 1) <= INT32_MAX, MSA_ERR_INVALID_ARG, "%s: too many rows for one call", who);
   MSA_REQUIRE(ldk >= n && ldv >= n && ldk % 8 == 0 && ldv % 8 == 0, MSA_ERR_INVALID_ARG,
               "%s: row strides must be multiples of 8 of at least kv_heads * hd", who);
   return MSA_OK;
@@ -197,20 +433,6 @@ int msa_paged_check(const msa_paged_cache* c, const msa_paged_batch* b, const ch
   return MSA_OK;
 }
 
-#define DISPATCH(kernel)                                                                                     \
-  do {                                                                                                       \
-    const dim3 grid((unsigned)b->M, (unsigned)((c->kv_heads + 3) / 4));                                      \
-    if (c->dtype == MSA_F16) {                                                                               \
-      if (c->format == MSA_PAGES_SAME) hipLaunchKernelGGL((kernel<MSA_F16, PG_F16>), grid, dim3(256), 0, s, a);   \
-      else if (c->format == MSA_PAGES_E4M3) hipLaunchKernelGGL((kernel<MSA_F16, PG_E4M3>), grid, dim3(256), 0, s, a); \
-      else hipLaunchKernelGGL((kernel<MSA_F16, PG_I8>), grid, dim3(256), 0, s, a);                           \
-    } else {                                                                                                 \
-      if (c->format == MSA_PAGES_SAME) hipLaunchKernelGGL((kernel<MSA_BF16, PG_BF16>), grid, dim3(256), 0, s, a); \
-      else if (c->format == MSA_PAGES_E4M3) hipLaunchKernelGGL((kernel<MSA_BF16, PG_E4M3>), grid, dim3(256), 0, s, a); \
-      else hipLaunchKernelGGL((kernel<MSA_BF16, PG_I8>), grid, dim3(256), 0, s, a);                          \
-    }                                                                                                        \
-  } while (0)
-
 extern "C" int msa_paged_append(const msa_paged_cache* c, const msa_paged_batch* b, const void* k, int64_t ldk, const void* v,
                                 int64_t ldv, void* stream) {
   const int rc = check_rows(c, b, k, ldk, v, ldv, "msa_paged_append");
@@ -218,7 +440,7 @@ extern "C" int msa_paged_append(const msa_paged_cache* c, const msa_paged_batch*
   if (b->M == 0 || b->nseq == 0 || b->max_count == 0) return MSA_OK;
   hipStream_t s = (hipStream_t)stream;
   const PagedRows a = {*c, *b, k, v, nullptr, nullptr, ldk, ldv, paged_log2(c->page)};
-  DISPATCH(append_rows_kernel);
+  launch_rows(a, true, s);
   MSA_CHECK_LAUNCH("msa_paged_append");
   return MSA_OK;
 }
@@ -230,7 +452,7 @@ extern "C" int msa_paged_read(const msa_paged_cache* c, const msa_paged_batch* b
   if (b->M == 0 || b->nseq == 0 || b->max_count == 0) return MSA_OK;
   hipStream_t s = (hipStream_t)stream;
   const PagedRows a = {*c, *b, nullptr, nullptr, k, v, ldk, ldv, paged_log2(c->page)};
-  DISPATCH(read_rows_kernel);
+  launch_rows(a, false, s);
   MSA_CHECK_LAUNCH("msa_paged_read");
   return MSA_OK;
 }
