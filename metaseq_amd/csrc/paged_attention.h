@@ -156,6 +156,15 @@ struct PaTiles {
   __device__ __forceinline__ int tile(int i) const { return i < head ? i : first + i - head; }
 };
 
+// pages of a tile's four groups of sixteen keys, -1: none
+struct PtPages {
+  int a, b, c, d;
+  __device__ __forceinline__ int of(int g16) const {
+    const int w = a, x = b, y = c, z = d;
+    return g16 < 2 ? (g16 < 1 ? w : x) : (g16 < 3 ? y : z);
+  }
+};
+
 template <int F, int HD, int RT>
 __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a) {
   typedef PaFormat<F> X;
@@ -243,18 +252,25 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
   }
   int E = -127;  // largest exponent of values met (8 bits)
 
-  // ---- where tile i's keys are.  As a source of K a lane has keys of quad n16 / 4, as one of V of its own quad ----
-  const int32_t* table = a.table + (int64_t)s * a.table_stride;
-  auto look = [&](int i, int q) {  // page of quad q's keys of tile i (clamped past the end: those are masked)
-    const int block = (tiles.tile(i) * KT + q * KQ) >> a.page_log2;
-    return block < a.blocks ? table[block] : -1;
+  // ---- tiles.  As a source of K a lane has keys of quad n16 / 4, as one of V of its own quad.  Keys and values are
+  // requested a tile ahead, each into the registers that the matrix instructions have just read ----
+  const pg_uniform_i32* table = (const pg_uniform_i32*)(uintptr_t)(a.table + (int64_t)s * a.table_stride);
+  // page of the sixteen keys g16 of tile i, -1 where there is none
+  auto look = [&](int i, int g16) {
+    const int block = (tiles.tile(i) * KT + g16 * 16) >> a.page_log2;
+    const int pg = table[min(block, a.blocks - 1)];
+    return block < a.blocks && (unsigned)pg < (unsigned)a.pages ? pg : -1;
   };
+  auto look4 = [&](int i) {
+    i = min(i, it_end - 1);
+    return PtPages{look(i, 0), look(i, 1), B8 ? look(i, 2) : 0, B8 ? look(i, 3) : 0};
+  };
+  auto of_quad = [](PtPages pg, int q) { return B8 ? pg.of(q) : pg.of(q >> 1); };
   const int64_t unit = (int64_t)page * HD * ES;  // bytes of a page and head
   pg_u4 kf[NT][KL], vf[DT];
-  auto load_k = [&](int i, int pg) {
-    const int key = tiles.tile(i) * KT + (n16 >> 2) * KQ + (n16 & 3);
-    const int64_t at = ((int64_t)(pg >= 0 && pg < a.pages ? pg : 0) * a.kv_heads + h) * unit + (int64_t)(key & (page - 1)) * (HD * ES) + quad * 16;
-    const char* base = (const char*)a.k_pages + at;
+  auto load_k = [&](int i, PtPages pages) {
+    const int key = tiles.tile(i) * KT + (n16 >> 2) * KQ + (n16 & 3), pg = of_quad(pages, n16 >> 2);
+    const char* base = (const char*)a.k_pages + ((int64_t)max(pg, 0) * a.kv_heads + h) * unit + (int64_t)(key & (page - 1)) * (HD * ES) + quad * 16;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -263,43 +279,45 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
                        ? __builtin_nontemporal_load((const pg_u4*)(base + t * 4 * HD * ES + c * 64))
                        : pg_u4{0, 0, 0, 0};
   };
-  auto load_v = [&](int i, int pg) {
-    const int key = tiles.tile(i) * KT + quad * KQ;
-    const int64_t at = ((int64_t)(pg >= 0 && pg < a.pages ? pg : 0) * a.kv_heads + h) * unit + ((int64_t)n16 * page + (key & (page - 1))) * ES;
-    const char* base = (const char*)a.v_pages + at;
+  auto load_v = [&](int i, PtPages pages) {
+    const int key = tiles.tile(i) * KT + quad * KQ, pg = of_quad(pages, quad);
+    const char* base = (const char*)a.v_pages + ((int64_t)max(pg, 0) * a.kv_heads + h) * unit + (n16 * page + (key & (page - 1))) * ES;
 #pragma unroll
-    for (int d = 0; d < DT; ++d) vf[d] = __builtin_nontemporal_load((const pg_u4*)(base + (int64_t)d * 16 * page * ES));
+    for (int d = 0; d < DT; ++d) vf[d] = __builtin_nontemporal_load((const pg_u4*)(base + d * 16 * page * ES));
   };
-  // exponents of the quad's keys
-  pg_u4 kx, vx;
-  auto load_x = [&](int i, int pg) {
-    const int key = tiles.tile(i) * KT + quad * KQ;
-    const int64_t at = ((int64_t)(pg >= 0 && pg < a.pages ? pg : 0) * a.kv_heads + h) * page + (key & (page - 1));
+  pg_u4 kx, vx;  // exponents of the quad's keys
+  auto load_x = [&](int i, PtPages pages) {
+    const int key = tiles.tile(i) * KT + quad * KQ, pg = of_quad(pages, quad);
+    const int64_t at = ((int64_t)max(pg, 0) * a.kv_heads + h) * page + (key & (page - 1));
     kx = *(const pg_u4*)(a.k_exp + at);
     vx = *(const pg_u4*)(a.v_exp + at);
   };
   auto byte_of = [](pg_u4 w, int i) { return (int)(int8_t)(w[i >> 2] >> ((i & 3) * 8)); };
 
-  for (int i = split * per + wave; i < it_end; i += PA_NW) {
-    const int pk = look(i, n16 >> 2), pv = look(i, quad);
-    load_k(i, pk);
-    load_v(i, pv);
-    if (B8) load_x(i, pv);
+  int i = split * per + wave;
+  PtPages pg = {-1, -1, -1, -1}, next = pg;  // of this tile and the wave's next one
+  if (i < it_end) {
+    pg = look4(i);
+    next = look4(i + PA_NW);
+    load_k(i, pg);
+    if (B8) load_x(i, pg);
+    load_v(i, pg);
+  }
+#pragma unroll 1
+  for (; i < it_end; i += PA_NW) {
     const int key0 = tiles.tile(i) * KT;  // of the tile
     const int kq = key0 + quad * KQ;      // of the quad
-    const bool here = pv >= 0 && pv < a.pages;
+    const bool there = of_quad(pg, quad) >= 0;
+    const bool more = i + PA_NW < it_end;
     // every row sees every key of the tile
     const bool whole = key0 + KT - 1 <= p_lo && (a.window <= 0 || key0 > p_hi - a.window || key0 + KT <= a.sinks) &&
-                       __ballot(!here) == 0;
-    // whether any row sees the key
-    auto any_sees = [&](int key) {
-      return here && key <= p_hi && (a.window <= 0 || key > p_lo - a.window || key < a.sinks);
-    };
+                       (pg.a | pg.b | pg.c | pg.d) >= 0;
+    // the quad's keys that some row sees
+    const uint32_t seen = whole ? ~0u : there ? pa_seen<KQ>(kq, p_lo, p_hi, a.window, a.sinks) : 0;
     if (B8) {
       int most = -127;
 #pragma unroll
-      for (int j = 0; j < KQ; ++j)
-        if (whole || any_sees(kq + j)) most = max(most, byte_of(vx, j));
+      for (int j = 0; j < KQ; ++j) most = max(most, (seen >> j) & 1 ? byte_of(vx, j) : -127);
       if (__ballot(most > E)) {
         most = max(most, __shfl_xor(most, 16, MSA_WAVE));
         most = max(most, __shfl_xor(most, 32, MSA_WAVE));
@@ -313,30 +331,38 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
         E = to;
       }
     }
+    float z[RT][KQ];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float4_t sc[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) sc[rt] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < KL; ++c)
+#pragma unroll
+        for (int e = 0; e < HALVES; ++e) {
+          const pg_u4 k = pa_operand<F>(kf[t][c], e);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) sc[rt] = pa_mfma<F>(k, qf[rt][c][e], sc[rt]);
+        }
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[rt][t * 4 + e] = sc[rt][e];
+    }
+    if (more) load_k(i + PA_NW, next);
     pg_u4 pf[RT][HALVES];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      float4_t sc[NT];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        sc[t] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < KL; ++c)
-#pragma unroll
-          for (int e = 0; e < HALVES; ++e) sc[t] = pa_mfma<F>(pa_operand<F>(kf[t][c], e), qf[rt][c][e], sc[t]);
-      }
+      const uint32_t sees = there ? pa_seen<KQ>(kq, pn[rt], pn[rt], a.window, a.sinks) : 0;
       float top = -INFINITY;
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int j = t * 4 + e, key = kq + j;
-          float z = sc[t][e] * qs[rt];
-          if (B8) z = ldexpf(z, byte_of(kx, j));
-          if (!whole && !(here && key <= pn[rt] && (a.window <= 0 || key > pn[rt] - a.window || key < a.sinks))) z = -INFINITY;
-          sc[t][e] = z;
-          top = fmaxf(top, z);
-        }
+      for (int j = 0; j < KQ; ++j) {
+        if (B8) z[rt][j] = ldexpf(z[rt][j], byte_of(kx, j));
+        z[rt][j] = (sees >> j) & 1 ? z[rt][j] : -INFINITY;
+        top = fmaxf(top, z[rt][j]);
+      }
+      top *= qs[rt];
       if (__ballot(top > m[rt] + PA_LAZY)) {  // (m = -inf: any score)
         const float to = fmaxf(m[rt], pa_quads_max(top));
         const float w = m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rt] - to);
@@ -347,14 +373,13 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[rt][d][e] *= w;
       }
-      const float off = m[rt] == -INFINITY ? 0.f : m[rt];
+      const float off = (m[rt] == -INFINITY ? 0.f : m[rt]) - (B8 ? 0.f : X::SHIFT);
       float p[KQ], sum = 0.f;
 #pragma unroll
       for (int j = 0; j < KQ; ++j) {
-        p[j] = __builtin_amdgcn_exp2f(sc[j >> 2][j & 3] - off);
+        p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[rt][j], qs[rt], -off));
         sum += p[j];
-        if (B8) p[j] = ldexpf(p[j], (whole || any_sees(kq + j) ? byte_of(vx, j) : -127) - E + (int)X::SHIFT);
-        else if (X::SHIFT != 0.f) p[j] *= exp2f(X::SHIFT);
+        if (B8) p[j] = ldexpf(p[j], ((seen >> j) & 1 ? byte_of(vx, j) : -127) - E + (int)X::SHIFT);
       }
       l[rt] += sum;
 #pragma unroll
@@ -372,41 +397,41 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
         }
       }
     }
+    if (B8 && more) load_x(i + PA_NW, next);
     if (!whole) {
       // Keys that no row sees may hold anything: their values are taken as zeros.  A value that is not finite at a key
       // that some rows see and others do not must reach those rows only (0 times infinity is NaN): it is left out of
       // the product, and products with ones in the places of infinities and NaN say which rows it reaches.
-      uint32_t seen = 0;
+      pg_u4 keep;
 #pragma unroll
-      for (int j = 0; j < KQ; ++j) seen |= any_sees(kq + j) ? 1u << j : 0;
+      for (int k = 0; k < 4; ++k) keep[k] = pa_keep<F>(~0u, seen >> (k * (KQ / 4)));
       bool odd = false;
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
+      for (int d = 0; d < DT; ++d) {
+        vf[d] &= keep;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          vf[d][i] = pa_keep<F>(vf[d][i], seen >> (i * (KQ / 4)));
-          odd |= pa_not_finite<F>(vf[d][i], 0) != 0;
-        }
-      if (__ballot(odd)) {
+        for (int k = 0; k < 4; ++k) odd |= pa_not_finite<F>(vf[d][k], 0) != 0;
+      }
+      if (F != PG_I8 && __ballot(odd)) {
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
 #pragma unroll 1
           for (int kind = 1; kind <= 3; ++kind) {
             pg_u4 ones;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) ones[i] = pa_not_finite<F>(vf[d][i], kind);
+            for (int k = 0; k < 4; ++k) ones[k] = pa_not_finite<F>(vf[d][k], kind);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
               float4_t hit = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
               for (int e = 0; e < HALVES; ++e) hit = pa_mfma<F>(pa_operand<F>(ones, e), pf[rt][e], hit);
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (hit[i] != 0.f) acc[rt][d][i] += kind == 1 ? INFINITY : kind == 2 ? -INFINITY : NAN;
+              for (int k = 0; k < 4; ++k)
+                if (hit[k] != 0.f) acc[rt][d][k] += kind == 1 ? INFINITY : kind == 2 ? -INFINITY : NAN;
             }
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) vf[d][i] = pa_finite<F>(vf[d][i]);
+          for (int k = 0; k < 4; ++k) vf[d][k] = pa_finite<F>(vf[d][k]);
         }
       }
     }
@@ -418,6 +443,9 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) acc[rt][d] = pa_mfma<F>(v, pf[rt][e], acc[rt][d]);
       }
+    if (more) load_v(i + PA_NW, next);
+    pg = next;
+    next = look4(i + 2 * PA_NW);
   }
 
   // ---- the waves' sums: one row tile at a time through LDS, added in the waves' order ----
@@ -433,7 +461,7 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
       for (int d = 0; d < DT; ++d) {
         float4_t v = acc[rt][d];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = B8 ? ldexpf(v[i], E - (int)X::SHIFT) : X::SHIFT != 0.f ? v[i] * exp2f(-X::SHIFT) : v[i];
+        for (int k = 0; k < 4; ++k) v[k] = B8 ? ldexpf(v[k], E - (int)X::SHIFT) : v[k];
         *(float4_t*)&s_acc[wave][n16][d * 16 + quad * 4] = v;
       }
     }
@@ -515,15 +543,6 @@ __device__ __forceinline__ float16_t pt_mfma(pg_u4 a, pg_u4 b, float16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
 }
-
-// pages of a tile's four groups of sixteen keys, -1: none
-struct PtPages {
-  int a, b, c, d;
-  __device__ __forceinline__ int of(int g16) const {
-    const int w = a, x = b, y = c, z = d;
-    return g16 < 2 ? (g16 < 1 ? w : x) : (g16 < 3 ? y : z);
-  }
-};
 
 template <int F, int HD>
 __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kernel(PagedAttention a) {

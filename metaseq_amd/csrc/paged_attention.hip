@@ -11,36 +11,54 @@ PAGED_FORMAT(i8)
 
 namespace {
 
-// One wave per (row, query head): out = sum of the splits' sums, each relative to its own maximum.
-// `few`, `many`: splits of the sequences of either kernel; 1: it wrote its outputs itself.
-__global__ __launch_bounds__(64) void paged_combine_kernel(PagedAttention a, int hd, int few, int many) {
-  const int lane = threadIdx.x, r = blockIdx.x, head = blockIdx.y;
+// out = sum of the splits' sums, each relative to its own maximum.  Workgroup = (row, query head); groups of hd / 4 threads take
+// every so manieth split, and their sums are added in the groups' order.  `few`, `many`: splits of the sequences of either
+// kernel; 1: it wrote its outputs itself.
+constexpr int PC_THREADS = 256;
+__global__ __launch_bounds__(PC_THREADS) void paged_combine_kernel(PagedAttention a, int hd, int few, int many) {
+  __shared__ __attribute__((aligned(16))) float s_o[PC_THREADS][4];
+  __shared__ float s_l[PC_THREADS];
+  const int lane = threadIdx.x & 63, r = blockIdx.x, head = blockIdx.y;
   const int s = __builtin_amdgcn_readfirstlane(paged_sequence_of(a.seq_start, a.nseq, r));
   if (s >= a.nseq || r >= a.seq_start[a.nseq] || a.seq_pos[s] < 0 || a.seq_start[s] < 0 || r - a.seq_start[s] >= a.max_count) return;
   const int count = min(min(a.seq_start[s + 1], a.M) - a.seq_start[s], a.max_count);
   const int splits = count * (a.heads / a.kv_heads) <= a.few ? few : many;
   if (splits == 1) return;
-  const float* part = a.partial + ((int64_t)r * a.heads + head) * splits * (hd + 4);
+  const int stride = hd + 4, columns = hd / 4, groups = PC_THREADS / columns;
+  const float* part = a.partial + ((int64_t)r * a.heads + head) * splits * stride;
   float top = -INFINITY;
-  for (int i = lane; i < splits; i += 64) top = fmaxf(top, part[(int64_t)i * (hd + 4) + hd]);
+  for (int i = lane; i < splits; i += 64) top = fmaxf(top, part[i * stride + hd]);
   top = wave_max(top);
   const float off = top == -INFINITY ? 0.f : top;
-  float o[4] = {0.f, 0.f, 0.f, 0.f}, total = 0.f;
-  for (int i = 0; i < splits; ++i) {
-    const float* p = part + (int64_t)i * (hd + 4);
-    const float w = __builtin_amdgcn_exp2f(p[hd] - off);
-    total += w * p[hd + 1];
+  const int g = threadIdx.x / columns, c = threadIdx.x - g * columns;
+  float4_t o = {0.f, 0.f, 0.f, 0.f};
+  float total = 0.f;
+  if (g < groups) {
+#pragma unroll 4
+    for (int i = g; i < splits; i += groups) {
+      const float4_t v = *(const float4_t*)(part + i * stride + c * 4);
+      const float w = __builtin_amdgcn_exp2f(part[i * stride + hd] - off);
+      total += w * part[i * stride + hd + 1];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (lane * 4 < hd) o[k] += w * p[lane * 4 + k];
+      for (int k = 0; k < 4; ++k) o[k] += w * v[k];
+    }
   }
-  if (lane * 4 >= hd) return;
+  *(float4_t*)s_o[threadIdx.x] = o;
+  s_l[threadIdx.x] = total;
+  __syncthreads();
+  if ((int)threadIdx.x >= columns) return;
+  for (int i = 1; i < groups; ++i) {
+    const float4_t v = *(const float4_t*)s_o[i * columns + c];
+    total += s_l[i * columns + c];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] += v[k];
+  }
   const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
   uint16_t w[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k)
     w[k] = a.bf16 ? __builtin_bit_cast(uint16_t, (bf16_t)(o[k] * inv)) : __builtin_bit_cast(uint16_t, (half_t)(o[k] * inv));
-  const int d = head * hd + lane * 4;
+  const int d = head * hd + c * 4;
   const int64_t at = a.out_mb > 0 ? packed_act_offset(r, d, a.out_mb) : (int64_t)r * a.ldo + d;
   *(pg_u2*)((uint16_t*)a.out + at) = pg_u2{(uint32_t)w[0] | (uint32_t)w[1] << 16, (uint32_t)w[2] | (uint32_t)w[3] << 16};
 }
@@ -166,7 +184,7 @@ extern "C" int msa_paged_attention(const msa_paged_cache* c, const msa_paged_bat
     MSA_CHECK_LAUNCH("msa_paged_attention (rows)");
   }
   if (p.splits > 1 || p.tile_splits > 1) {
-    hipLaunchKernelGGL(paged_combine_kernel, dim3((unsigned)b->M, (unsigned)a->heads), dim3(64), 0, s, k, c->hd,
+    hipLaunchKernelGGL(paged_combine_kernel, dim3((unsigned)b->M, (unsigned)a->heads), dim3(PC_THREADS), 0, s, k, c->hd,
                        p.row_tiles > 0 ? p.splits : 1, p.tile_blocks > 0 ? p.tile_splits : 1);
     MSA_CHECK_LAUNCH("msa_paged_attention (splits)");
   }

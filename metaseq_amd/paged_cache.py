@@ -34,6 +34,7 @@ class PagedBatch:
     def __init__(self, c, rows, seq_start, seq_pos, table):
         self.c, self.rows, self.seq_start, self.seq_pos, self.table = c, rows, seq_start, seq_pos, table
         self.by_ref = ctypes.byref(c)
+        self.workspaces = {}   # bytes that attention over such heads and pages asks for
 
     @property
     def key_bound(self):
@@ -70,6 +71,7 @@ class PagedCache:
         self.pages, self.kv_heads, self.page, self.head_dim = pages, kv_heads, page, hd
         self.device = k_pages.device
         self._lib = _capi.load()
+        self._scale = 1.0 / math.sqrt(hd)
         self._c = {}
         for dtype, code in _DTYPES.items():
             if eight or dtype == k_pages.dtype:
@@ -136,12 +138,12 @@ class PagedCache:
 
     def _rows(self, name, t, rows, heads, copy):
         """``t`` as rows of heads, one behind the other, that the kernels can read or write in place."""
-        if tuple(t.shape) != (rows, heads, self.head_dim) or t.device != self.device:
+        if t.shape != (rows, heads, self.head_dim) or t.device != self.device:
             raise ValueError("%s must be [%d, %d, %d] on %s, not %s on %s"
                              % (name, rows, heads, self.head_dim, self.device, list(t.shape), t.device))
-        _, sh, sd = t.stride()
+        sr, sh, sd = t.stride()
         if sd == 1 and (heads == 1 or sh == self.head_dim) and t.data_ptr() % 16 == 0 and \
-                (rows < 2 or (t.stride(0) % 8 == 0 and t.stride(0) >= heads * self.head_dim)):
+                (rows < 2 or (sr % 8 == 0 and sr >= heads * self.head_dim)):
             return t
         if not copy:
             raise ValueError("%s must have its heads one behind the other, 16-byte aligned, rows a multiple of 8 apart"
@@ -153,11 +155,13 @@ class PagedCache:
         return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
 
     def _run(self, fn, *args):
-        if torch.cuda.current_device() == self.device.index:
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+        at = self.device.index
+        stream = torch._C._cuda_getCurrentRawStream(at)   # (torch.cuda.current_stream without its object)
+        if torch._C._cuda_getDevice() == at:
+            rc = fn(*args, stream)
         else:
             with torch.cuda.device(self.device):
-                rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+                rc = fn(*args, stream)
         if rc:
             _capi.check(rc, self._lib)
 
@@ -203,11 +207,15 @@ class PagedCache:
         else:
             self._rows("out", out, batch.rows, heads, False)
         a = _capi.PagedAttentionArgs(heads, q.data_ptr(), self._ld(q), out.data_ptr(), self._ld(out), 0, window, sinks,
-                                     1.0 / math.sqrt(self.head_dim) if scale is None else scale, None, 0)
+                                     self._scale if scale is None else scale, None, 0)
         ref = ctypes.byref(a)
-        need = self._lib.msa_paged_attention_workspace_bytes(c, batch.by_ref, ref)
-        if need < 0:
-            _capi.check(need, self._lib)
+        what = (self.kv_heads, self.head_dim, self.k_pages.dtype, heads, window, sinks)
+        need = batch.workspaces.get(what)
+        if need is None:
+            need = self._lib.msa_paged_attention_workspace_bytes(c, batch.by_ref, ref)
+            if need < 0:
+                _capi.check(need, self._lib)
+            batch.workspaces[what] = need
         if need:
             # (from torch's allocator, so that two captured graphs never share one)
             ws = torch.empty(need, dtype=torch.uint8, device=self.device)
