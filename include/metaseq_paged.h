@@ -38,10 +38,10 @@ typedef struct {
  * outputs stay as they were).  Position p of sequence s is in page table[s * table_stride + p / page]; positions
  * whose entry is outside 0 .. pages - 1, or beyond the `blocks` entries of a sequence, are nowhere: they are not written,
  * read back as zeros and seen by no row.  max_count: no sequence has more rows (those that it has beyond are left
- * alone); key_bound: no row's position reaches it (a hint: how keys are split follows from it, results up to
+ * alone); min_count: no sequence that has rows has fewer (0: not known); key_bound: no row's position reaches it (a hint: how keys are split follows from it, results up to
  * rounding do not). */
 typedef struct {
-  int M, nseq, max_count, key_bound, blocks;
+  int M, nseq, max_count, min_count, key_bound, blocks;
   int64_t table_stride;
   const int32_t *seq_start, *seq_pos, *table;
 } msa_paged_batch;

@@ -248,7 +248,7 @@ MSA_F16 = 2
 MSA_PAGES_SAME, MSA_PAGES_E4M3, MSA_PAGES_INT8 = 0, 1, 2
 PagedCacheC = _struct("PagedCacheC", "msa_paged_cache", (c_int, "dtype format kv_heads hd page pages"),
                       (c_void_p, "k_pages v_pages k_exp v_exp"))
-PagedBatchC = _struct("PagedBatchC", "msa_paged_batch", (c_int, "M nseq max_count key_bound blocks"),
+PagedBatchC = _struct("PagedBatchC", "msa_paged_batch", (c_int, "M nseq max_count min_count key_bound blocks"),
                       (c_int64, "table_stride"), (c_void_p, "seq_start seq_pos table"))
 PagedAttentionArgs = _struct(
     "PagedAttentionArgs", "msa_paged_attention_args", (c_int, "heads"), (c_void_p, "q"), (c_int64, "ldq"),

@@ -176,12 +176,14 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
   constexpr int DT = HD / 16;                  // 16-dimension tiles of O^T
   constexpr int LDO = HD + 4;
   __shared__ __attribute__((aligned(16))) float s_acc[PA_NW][16][LDO];
+  static_assert(16 * LDO * 4 >= HD * KT * ES, "a tile's values of one wave");
   __shared__ float s_m[PA_NW][16], s_l[PA_NW][16];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n16 = lane & 15, quad = lane >> 4;
-  const int s = blockIdx.x / a.row_blocks, rb = blockIdx.x - s * a.row_blocks;
-  const int h = blockIdx.y, split = blockIdx.z;
+  // (the heads of a sequence next to one another, as they are in its pages)
+  const int srb = blockIdx.x / a.kv_heads, h = blockIdx.x - srb * a.kv_heads, split = blockIdx.y;
+  const int s = srb / a.row_blocks, rb = srb - s * a.row_blocks;
   const int group = a.heads / a.kv_heads;
   const pg_uniform_i32* seq_start = (const pg_uniform_i32*)(uintptr_t)a.seq_start;
   const int row0 = seq_start[s], pos = ((const pg_uniform_i32*)(uintptr_t)a.seq_pos)[s];
@@ -193,8 +195,7 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
   const int p_hi = (int)min((int64_t)pos + (min(rho0 + 16 * RT, rows) - 1) / group, (int64_t)limit);
   const PaTiles<KT> tiles(p_lo, p_hi, a.window, a.sinks);
   // this split's tiles, every PA_NW-th of them this wave's
-  const int per = (tiles.n + a.splits - 1) / a.splits;
-  const int it_end = min(tiles.n, (split + 1) * per);
+  const int per = (tiles.n + a.splits - 1) / a.splits, it_end = min(tiles.n, (split + 1) * per);
 
   // ---- queries: B operand, row n16 of row tile rt, the dimensions that the lane's loads of K have ----
   pg_u4 qf[RT][KL][HALVES];
@@ -253,7 +254,10 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
   int E = -127;  // largest exponent of values met (8 bits)
 
   // ---- tiles.  As a source of K a lane has keys of quad n16 / 4, as one of V of its own quad.  Keys and values are
-  // requested a tile ahead, each into the registers that the matrix instructions have just read ----
+  // requested a tile ahead, each into the registers that the matrix instructions have just read.  (Keys of 16 bits past the
+  // caches, nothing else: the two halves of a line of values are different waves', and lines of 8-bit keys are two
+  // instructions'.  32 sequences of 32 heads over 640 to 1281 keys, us: 135 with everything past them, 116 with nothing, 98
+  // so; one of 8 heads over 131072 in int8 55, 46 with nothing) ----
   const pg_uniform_i32* table = (const pg_uniform_i32*)(uintptr_t)(a.table + (int64_t)s * a.table_stride);
   // page of the sixteen keys g16 of tile i, -1 where there is none
   auto look = [&](int i, int g16) {
@@ -276,14 +280,15 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
 #pragma unroll
       for (int c = 0; c < KL; ++c)
         kf[t][c] = (c + 1) * CD <= HD || quad * (CD / 4) + c * CD < HD
-                       ? __builtin_nontemporal_load((const pg_u4*)(base + t * 4 * HD * ES + c * 64))
+                       ? B8 ? *(const pg_u4*)(base + t * 4 * HD * ES + c * 64)
+                            : __builtin_nontemporal_load((const pg_u4*)(base + t * 4 * HD * ES + c * 64))
                        : pg_u4{0, 0, 0, 0};
   };
   auto load_v = [&](int i, PtPages pages) {
     const int key = tiles.tile(i) * KT + quad * KQ, pg = of_quad(pages, quad);
     const char* base = (const char*)a.v_pages + ((int64_t)max(pg, 0) * a.kv_heads + h) * unit + (n16 * page + (key & (page - 1))) * ES;
 #pragma unroll
-    for (int d = 0; d < DT; ++d) vf[d] = __builtin_nontemporal_load((const pg_u4*)(base + d * 16 * page * ES));
+    for (int d = 0; d < DT; ++d) vf[d] = *(const pg_u4*)(base + d * 16 * page * ES);
   };
   pg_u4 kx, vx;  // exponents of the quad's keys
   auto load_x = [&](int i, PtPages pages) {
@@ -303,12 +308,13 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
     if (B8) load_x(i, pg);
     load_v(i, pg);
   }
-#pragma unroll 1
-  for (; i < it_end; i += PA_NW) {
+  // MORE: there is a next tile of this wave's.  (The last one has a copy of its own: behind a branch around the requests
+  // every wait would be for all of them.)
+  auto step = [&](auto more) {
+    constexpr bool MORE = decltype(more)::value;
     const int key0 = tiles.tile(i) * KT;  // of the tile
     const int kq = key0 + quad * KQ;      // of the quad
     const bool there = of_quad(pg, quad) >= 0;
-    const bool more = i + PA_NW < it_end;
     // every row sees every key of the tile
     const bool whole = key0 + KT - 1 <= p_lo && (a.window <= 0 || key0 > p_hi - a.window || key0 + KT <= a.sinks) &&
                        (pg.a | pg.b | pg.c | pg.d) >= 0;
@@ -350,7 +356,7 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
 #pragma unroll
         for (int e = 0; e < 4; ++e) z[rt][t * 4 + e] = sc[rt][e];
     }
-    if (more) load_k(i + PA_NW, next);
+    if (MORE) load_k(i + PA_NW, next);
     pg_u4 pf[RT][HALVES];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -397,11 +403,11 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
         }
       }
     }
-    if (B8 && more) load_x(i + PA_NW, next);
+    if (B8 && MORE) load_x(i + PA_NW, next);
     if (!whole) {
       // Keys that no row sees may hold anything: their values are taken as zeros.  A value that is not finite at a key
-      // that some rows see and others do not must reach those rows only (0 times infinity is NaN): it is left out of
-      // the product, and products with ones in the places of infinities and NaN say which rows it reaches.
+      // that some rows see and others do not must reach those rows only (0 times infinity is NaN): it is added to those
+      // and left out of the product.
       pg_u4 keep;
 #pragma unroll
       for (int k = 0; k < 4; ++k) keep[k] = pa_keep<F>(~0u, seen >> (k * (KQ / 4)));
@@ -412,27 +418,32 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
 #pragma unroll
         for (int k = 0; k < 4; ++k) odd |= pa_not_finite<F>(vf[d][k], 0) != 0;
       }
-      if (F != PG_I8 && __ballot(odd)) {
+      if (F != PG_I8 && __ballot(odd)) {  // (an infinity or a NaN times a probability is itself)
+        char* vt = (char*)s_acc[wave];    // [dimension][key]; not used before the end
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
+        for (int d = 0; d < DT; ++d) *(pg_u4*)(vt + ((d * 16 + n16) * KT + quad * KQ) * ES) = vf[d];
 #pragma unroll 1
-          for (int kind = 1; kind <= 3; ++kind) {
-            pg_u4 ones;
+        for (int j = 0; j < KT; ++j) {
+          const char* at = vt + (quad * 4 * KT + j) * ES;
+          const bool anywhere = of_quad(pg, j / KQ) >= 0;
+          bool mine[RT];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) ones[k] = pa_not_finite<F>(vf[d][k], kind);
+          for (int rt = 0; rt < RT; ++rt) mine[rt] = anywhere && pa_seen<1>(key0 + j, pn[rt], pn[rt], a.window, a.sinks);
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-              float4_t hit = {0.f, 0.f, 0.f, 0.f};
+          for (int d = 0; d < DT; ++d)
 #pragma unroll
-              for (int e = 0; e < HALVES; ++e) hit = pa_mfma<F>(pa_operand<F>(ones, e), pf[rt][e], hit);
+            for (int k = 0; k < 4; ++k) {
+              const char* x = at + (d * 16 + k) * KT * ES;
+              const float f = B8 ? ((*(const uint8_t*)x & 0x7f) == 0x7f ? NAN : 0.f)
+                                 : F == PG_BF16 ? (float)*(const bf16_t*)x : (float)*(const half_t*)x;
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                if (hit[k] != 0.f) acc[rt][d][k] += kind == 1 ? INFINITY : kind == 2 ? -INFINITY : NAN;
+              for (int rt = 0; rt < RT; ++rt) acc[rt][d][k] += (mine[rt] & !(fabsf(f) < INFINITY)) ? f : 0.f;
             }
-          }
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
 #pragma unroll
           for (int k = 0; k < 4; ++k) vf[d][k] = pa_finite<F>(vf[d][k]);
-        }
       }
     }
 #pragma unroll
@@ -443,10 +454,15 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) acc[rt][d] = pa_mfma<F>(v, pf[rt][e], acc[rt][d]);
       }
-    if (more) load_v(i + PA_NW, next);
+    if (MORE) load_v(i + PA_NW, next);
+  };
+#pragma unroll 1
+  for (; i + PA_NW < it_end; i += PA_NW) {
+    step(std::true_type{});
     pg = next;
     next = look4(i + 2 * PA_NW);
   }
+  if (i < it_end) step(std::false_type{});
 
   // ---- the waves' sums: one row tile at a time through LDS, added in the waves' order ----
 #pragma unroll
@@ -466,8 +482,8 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
       }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < left * (HD / 4); i += PA_NW * 64) {
-      const int r = i / (HD / 4), d = (i - r * (HD / 4)) * 4;
+    for (int j = threadIdx.x; j < left * (HD / 4); j += PA_NW * 64) {
+      const int r = j / (HD / 4), d = (j - r * (HD / 4)) * 4;
       float to = -INFINITY;
 #pragma unroll
       for (int w = 0; w < PA_NW; ++w) to = fmaxf(to, s_m[w][r]);
@@ -477,7 +493,6 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
 #pragma unroll
       for (int w = 0; w < PA_NW; ++w) {
         const float f = __builtin_amdgcn_exp2f(s_m[w][r] - off);
-        // (a wave without keys has no sum, and its zeros take part in none that a NaN maximum would spoil)
         total += f * s_l[w][r];
         const float4_t v = *(const float4_t*)&s_acc[w][r][d];
 #pragma unroll
@@ -486,9 +501,9 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
       const int rho = rho0 + rt * 16 + r, t = rho / group, head = h * group + rho - t * group;
       const int64_t row = (int64_t)row0 + t;
       if (a.splits > 1) {
-        float* to_ = a.partial + ((row * a.heads + head) * a.splits + split) * (HD + 4);
-        *(float4_t*)(to_ + d) = o;
-        if (d == 0) to_[HD] = to, to_[HD + 1] = total;
+        float* part = a.partial + ((row * a.heads + head) * a.splits + split) * (HD + 4);
+        *(float4_t*)(part + d) = o;
+        if (d == 0) part[HD] = to, part[HD + 1] = total;
       } else {
         const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
         uint16_t w[4];
@@ -962,7 +977,7 @@ bool pa_launch_tiles(const PagedAttention& a, hipStream_t stream) {
 
 template <int F, int HD>
 void pa_launch_rows(const PagedAttention& a, int rt, hipStream_t stream) {
-  const dim3 grid((unsigned)((int64_t)a.nseq * a.row_blocks), (unsigned)a.kv_heads, (unsigned)a.splits);
+  const dim3 grid((unsigned)((int64_t)a.nseq * a.row_blocks * a.kv_heads), (unsigned)a.splits);
   if (rt == 1) hipLaunchKernelGGL((paged_rows_kernel<F, HD, 1>), grid, dim3(PA_NW * 64), 0, stream, a);
   else hipLaunchKernelGGL((paged_rows_kernel<F, HD, 2>), grid, dim3(PA_NW * 64), 0, stream, a);
 }

@@ -11,19 +11,19 @@ PAGED_FORMAT(i8)
 
 namespace {
 
-// out = sum of the splits' sums, each relative to its own maximum.  Workgroup = (row, query head); groups of hd / 4 threads take
-// every so manieth split, and their sums are added in the groups' order.  `few`, `many`: splits of the sequences of either
-// kernel; 1: it wrote its outputs itself.
+// out = sum of the splits' sums, each relative to its own maximum.  Workgroup = (token, query head); groups of hd / 4 threads
+// take every so manieth split, and their sums are added in the groups' order.  tokens: of the sequences of the wave kernel, at
+// most so many each; 0: every row of those of the tile kernel.
 constexpr int PC_THREADS = 256;
-__global__ __launch_bounds__(PC_THREADS) void paged_combine_kernel(PagedAttention a, int hd, int few, int many) {
+__global__ __launch_bounds__(PC_THREADS) void paged_combine_kernel(PagedAttention a, int hd, int tokens) {
   __shared__ __attribute__((aligned(16))) float s_o[PC_THREADS][4];
   __shared__ float s_l[PC_THREADS];
-  const int lane = threadIdx.x & 63, r = blockIdx.x, head = blockIdx.y;
-  const int s = __builtin_amdgcn_readfirstlane(paged_sequence_of(a.seq_start, a.nseq, r));
-  if (s >= a.nseq || r >= a.seq_start[a.nseq] || a.seq_pos[s] < 0 || a.seq_start[s] < 0 || r - a.seq_start[s] >= a.max_count) return;
-  const int count = min(min(a.seq_start[s + 1], a.M) - a.seq_start[s], a.max_count);
-  const int splits = count * (a.heads / a.kv_heads) <= a.few ? few : many;
-  if (splits == 1) return;
+  const int lane = threadIdx.x & 63, head = blockIdx.y, splits = a.splits;
+  const int s = tokens > 0 ? blockIdx.x / tokens : __builtin_amdgcn_readfirstlane(paged_sequence_of(a.seq_start, a.nseq, blockIdx.x));
+  if (s >= a.nseq) return;
+  const int row0 = a.seq_start[s], r = tokens > 0 ? row0 + (int)blockIdx.x - s * tokens : (int)blockIdx.x;
+  const int count = min(min(a.seq_start[s + 1], a.M) - row0, a.max_count);
+  if (a.seq_pos[s] < 0 || row0 < 0 || r - row0 >= count || (count * (a.heads / a.kv_heads) <= a.few) != (tokens > 0)) return;
   const int stride = hd + 4, columns = hd / 4, groups = PC_THREADS / columns;
   const float* part = a.partial + ((int64_t)r * a.heads + head) * splits * stride;
   float top = -INFINITY;
@@ -66,7 +66,7 @@ __global__ __launch_bounds__(PC_THREADS) void paged_combine_kernel(PagedAttentio
 // How a batch is taken: sequences of at most PA_FEW rows (token, query head) of a key/value head by the wave kernel, others
 // by tiles; each splits keys over workgroups where there are few of those.
 struct Plan {
-  int row_tiles, row_blocks, splits;      // wave kernel (row_tiles 0: not launched)
+  int row_tiles, row_blocks, splits;  // wave kernel (row_tiles 0: not launched)
   int tile_blocks, tile_splits, grouped;  // tile kernel (tile_blocks 0: not launched)
 };
 
@@ -82,19 +82,18 @@ Plan plan_of(const msa_paged_cache& c, const msa_paged_batch& b, const msa_paged
   Plan p = {0, 0, 1, 0, 1, 0};
   const int group = a.heads / c.kv_heads;
   const int64_t rows = (int64_t)b.max_count * group;
-  // whether every sequence has max_count rows
-  const bool even = (int64_t)b.nseq * b.max_count <= b.M;
   // keys that a row block can see
   auto keys_of = [&](int64_t tokens) {
     const int64_t span = (int64_t)a.window + a.sinks + tokens;
     return a.window > 0 && span < b.key_bound ? span : (int64_t)b.key_bound;
   };
-  if (rows <= PA_FEW || !even) {
+  if ((int64_t)b.min_count * group <= PA_FEW) {
     const int64_t most = rows < PA_FEW ? rows : PA_FEW;
     p.row_tiles = most <= 16 ? 1 : 2;
     p.row_blocks = (int)((most + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
     const int kt = c.format == MSA_PAGES_SAME ? 32 : 64;
-    p.splits = splits_of((int64_t)b.nseq * p.row_blocks * c.kv_heads, 1024, (keys_of(most) + kt - 1) / kt, PA_NW);
+    const int64_t units = (int64_t)b.nseq * p.row_blocks * c.kv_heads;
+    p.splits = splits_of(units, 512, (keys_of(most) + kt - 1) / kt, PA_NW);
   }
   if (rows > PA_FEW) {
     p.tile_blocks = (int)((rows + PT_BM - 1) / PT_BM);
@@ -154,7 +153,7 @@ extern "C" int msa_paged_attention(const msa_paged_cache* c, const msa_paged_bat
               "msa_paged_attention: the workspace has %lld bytes, %lld are needed", (long long)a->workspace_bytes, (long long)need);
   const Plan p = plan_of(*c, *b, *a);
   const int64_t units = (int64_t)b->nseq * c->kv_heads;
-  MSA_REQUIRE((int64_t)b->nseq * p.row_blocks <= INT32_MAX && (units + 7) * p.tile_blocks * p.tile_splits <= INT32_MAX,
+  MSA_REQUIRE((int64_t)b->nseq * PA_FEW <= INT32_MAX && units * p.row_blocks <= INT32_MAX && (units + 7) * p.tile_blocks * p.tile_splits <= INT32_MAX,
               MSA_ERR_INVALID_ARG, "msa_paged_attention: too many rows for one call");
   PagedAttention k = {a->q, c->k_pages, c->v_pages, c->k_exp, c->v_exp, b->seq_start, b->seq_pos, b->table, a->ldq, a->ldo,
                       b->table_stride, a->out, (float*)a->workspace, b->M, b->nseq, a->heads, c->kv_heads, c->pages,
@@ -162,6 +161,11 @@ extern "C" int msa_paged_attention(const msa_paged_cache* c, const msa_paged_bat
                       c->dtype == MSA_BF16, b->max_count, PA_FEW, p.grouped, a->scale};
   hipStream_t s = (hipStream_t)stream;
   const int format = paged_format(*c);
+  auto combine = [&](int tokens) {
+    if (k.splits == 1) return;
+    hipLaunchKernelGGL(paged_combine_kernel, dim3((unsigned)(tokens > 0 ? b->nseq * tokens : b->M), (unsigned)a->heads),
+                       dim3(PC_THREADS), 0, s, k, c->hd, tokens);
+  };
   if (p.tile_blocks > 0) {
     k.splits = p.tile_splits;
     k.row_blocks = p.tile_blocks;
@@ -170,6 +174,7 @@ extern "C" int msa_paged_attention(const msa_paged_cache* c, const msa_paged_bat
                     : format == PG_E4M3 ? msa_launch_paged_tiles_e4m3(k, c->hd, s)
                                         : msa_launch_paged_tiles_i8(k, c->hd, s);
     MSA_REQUIRE(ok, MSA_ERR_HIP, "msa_paged_attention: the kernel's LDS was refused");
+    combine(0);
     MSA_CHECK_LAUNCH("msa_paged_attention (tiles)");
   }
   if (p.row_tiles > 0) {
@@ -181,12 +186,9 @@ extern "C" int msa_paged_attention(const msa_paged_cache* c, const msa_paged_bat
       case PG_E4M3: msa_launch_paged_rows_e4m3(k, c->hd, p.row_tiles, s); break;
       default: msa_launch_paged_rows_i8(k, c->hd, p.row_tiles, s); break;
     }
+    const int few = PA_FEW / (a->heads / c->kv_heads);
+    combine(few < 1 ? 1 : few < b->max_count ? few : b->max_count);
     MSA_CHECK_LAUNCH("msa_paged_attention (rows)");
-  }
-  if (p.splits > 1 || p.tile_splits > 1) {
-    hipLaunchKernelGGL(paged_combine_kernel, dim3((unsigned)b->M, (unsigned)a->heads), dim3(PC_THREADS), 0, s, k, c->hd,
-                       p.row_tiles > 0 ? p.splits : 1, p.tile_blocks > 0 ? p.tile_splits : 1);
-    MSA_CHECK_LAUNCH("msa_paged_attention (splits)");
   }
   return MSA_OK;
 }

@@ -427,6 +427,7 @@ int msa_paged_check(const msa_paged_cache* c, const msa_paged_batch* b, const ch
               MSA_ERR_INVALID_ARG, "%s: pages and exponents must be 16-byte aligned", who);
   MSA_REQUIRE(b->M >= 0 && b->nseq >= 0 && b->nseq <= (1 << 20) && b->max_count >= 0 && b->key_bound >= 0, MSA_ERR_INVALID_ARG,
               "%s: negative sizes, or more than 2^20 sequences", who);
+  MSA_REQUIRE(b->min_count >= 0 && b->min_count <= b->max_count, MSA_ERR_INVALID_ARG, "%s: min_count must be 0 .. max_count", who);
   MSA_REQUIRE(b->blocks >= 1 && b->table_stride >= b->blocks && (int64_t)b->blocks * c->page <= INT32_MAX,
               MSA_ERR_INVALID_ARG, "%s: blocks must be positive, at most table_stride and 2^31 positions", who);
   MSA_REQUIRE(b->nseq == 0 || (b->seq_start && b->seq_pos && b->table), MSA_ERR_INVALID_ARG, "%s: null pointer", who);

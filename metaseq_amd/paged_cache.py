@@ -126,7 +126,8 @@ class PagedCache:
         if key_bound is not None:
             bound = int(key_bound)
         stride = table.stride(0) if table.shape[0] > 1 else table.shape[1]
-        c = _capi.PagedBatchC(start[-1], len(new), max(new, default=0), max(0, min(bound, span)), table.shape[1], stride,
+        c = _capi.PagedBatchC(start[-1], len(new), max(new, default=0), min((n for n in new if n), default=0),
+                              max(0, min(bound, span)), table.shape[1], stride,
                               seq_start.data_ptr(), seq_pos.data_ptr(), table.data_ptr())
         return PagedBatch(c, start[-1], seq_start, seq_pos, table)
 
