@@ -254,10 +254,9 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
   int E = -127;  // largest exponent of values met (8 bits)
 
   // ---- tiles.  As a source of K a lane has keys of quad n16 / 4, as one of V of its own quad.  Keys and values are
-  // requested a tile ahead, each into the registers that the matrix instructions have just read.  (Keys of 16 bits past the
-  // caches, nothing else: the two halves of a line of values are different waves', and lines of 8-bit keys are two
-  // instructions'.  32 sequences of 32 heads over 640 to 1281 keys, us: 135 with everything past them, 116 with nothing, 98
-  // so; one of 8 heads over 131072 in int8 55, 46 with nothing) ----
+  // requested a tile ahead, each into the registers that the matrix instructions have just read.  (Nothing past the caches: a
+  // line of keys is two instructions', one of values two tiles'.  32 sequences of 32 heads over 640 to 1281 keys in fp16, us:
+  // 135 with everything past them, 107 so) ----
   const pg_uniform_i32* table = (const pg_uniform_i32*)(uintptr_t)(a.table + (int64_t)s * a.table_stride);
   // page of the sixteen keys g16 of tile i, -1 where there is none
   auto look = [&](int i, int g16) {
@@ -280,8 +279,7 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
 #pragma unroll
       for (int c = 0; c < KL; ++c)
         kf[t][c] = (c + 1) * CD <= HD || quad * (CD / 4) + c * CD < HD
-                       ? B8 ? *(const pg_u4*)(base + t * 4 * HD * ES + c * 64)
-                            : __builtin_nontemporal_load((const pg_u4*)(base + t * 4 * HD * ES + c * 64))
+                       ? *(const pg_u4*)(base + t * 4 * HD * ES + c * 64)
                        : pg_u4{0, 0, 0, 0};
   };
   auto load_v = [&](int i, PtPages pages) {

@@ -187,6 +187,66 @@ __device__ __forceinline__ bool block_of(const PagedRows& a, int s, int i, Block
 template <int HD>
 constexpr int row_lanes() { return HD <= 64 ? 8 : HD <= 128 ? 16 : 32; }
 
+// Eight elements of a row that LR lanes share -> their codes and the row's exponent.  The largest magnitude is that of the
+// bits; rows that hold a NaN, or more than codes can stand for, take the way of single elements.
+template <int DT, int F, int LR>
+__device__ __forceinline__ pg_u2 quantise8(pg_u4 w, int& e) {
+  typedef typename Elem<DT>::T T;
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  constexpr uint32_t INF = DT == MSA_F16 ? 0x7c00 : 0x7f80;
+  auto of = [](uint32_t bits) { return (float)__builtin_bit_cast(T, (uint16_t)bits); };
+  auto across = [](float m) {
+#pragma unroll
+    for (int o = LR / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, MSA_WAVE));
+    return m;
+  };
+  u16x2 m2 = {0, 0};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) m2 = __builtin_elementwise_max(m2, __builtin_bit_cast(u16x2, w[j] & 0x7fff7fffu));
+  uint32_t bits = max((uint32_t)m2[0], (uint32_t)m2[1]);
+#pragma unroll
+  for (int o = LR / 2; o > 0; o >>= 1) bits = max(bits, (uint32_t)__shfl_xor((int)bits, o, MSA_WAVE));
+  const float cap = largest<DT, F>();
+  pg_u2 out;
+  if (__ballot(bits > INF || of(bits) > cap)) {
+    float x[8], most = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = of(w[j >> 1] >> ((j & 1) * 16));
+      most = fmaxf(most, magnitude(x[j]));
+    }
+    e = exponent_of<F>(fminf(across(most), cap));
+    const float f = inverse_power(e);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = (x[j] > cap ? cap : x[j] < -cap ? -cap : x[j]) * f;
+    out[0] = code2<F>(x[0], x[1]) | code2<F>(x[2], x[3]) << 16;
+    out[1] = code2<F>(x[4], x[5]) | code2<F>(x[6], x[7]) << 16;
+    return out;
+  }
+  e = exponent_of<F>(of(bits));
+  const float f = inverse_power(e);
+  if (F == PG_E4M3) {  // (gfx950's conversions from 16 bits with a scale lose the leading bit of subnormals)
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = of(w[j >> 1] >> ((j & 1) * 16)) * f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i], x[4 * i + 1], 0, false);
+      out[i] = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2], x[4 * i + 3], lo, true);
+    }
+    return out;
+  }
+  // int8: the last bits of x 2^-e + 1.5 2^23 are the integer, rounded by the addition (x 2^-e is exact)
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint32_t z[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) z[j] = __builtin_bit_cast(uint32_t, __builtin_fmaf(of(w[2 * i + (j >> 1)] >> ((j & 1) * 16)), f, 12582912.f));
+    out[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(z[3], z[2], 0x0c0c0400u), __builtin_amdgcn_perm(z[1], z[0], 0x0c0c0400u), 0x05040100u);
+  }
+  return out;
+}
+
 template <int DT, int F, int HD>
 __global__ __launch_bounds__(256) void append_block_kernel(PagedRows a, int blocks) {
   typedef typename Elem<DT>::T T;
@@ -194,9 +254,11 @@ __global__ __launch_bounds__(256) void append_block_kernel(PagedRows a, int bloc
   constexpr int STRIDE = HD * ES + 4;                  // of an LDS row: columns are read without bank conflicts
   constexpr int G = 16 / ES, NG = PB / G;              // positions of 16 bytes of a dimension
   __shared__ __attribute__((aligned(16))) char lds[PB * STRIDE];
-  const int s = blockIdx.x / blocks, h = blockIdx.y, lane = threadIdx.x % LR, r0 = threadIdx.x / LR;
+  // (the heads of a block next to one another: their pieces of a row are)
+  const int sb = blockIdx.x / a.c.kv_heads, h = blockIdx.x - sb * a.c.kv_heads, s = sb / blocks;
+  const int lane = threadIdx.x % LR, r0 = threadIdx.x / LR;
   Block b;
-  if (!block_of(a, s, blockIdx.x - s * blocks, b)) return;
+  if (!block_of(a, s, sb - s * blocks, b)) return;
   const int page = 1 << a.page_log2;
   pg_u4 k[N], v[N];
 #pragma unroll
@@ -223,59 +285,55 @@ __global__ __launch_bounds__(256) void append_block_kernel(PagedRows a, int bloc
       }
       continue;
     }
-    const float cap = largest<DT, F>();
-    float kx[8], vx[8], km = 0.f, vm = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      kx[j] = (float)__builtin_bit_cast(T, (uint16_t)(k[i][j >> 1] >> ((j & 1) * 16)));
-      vx[j] = (float)__builtin_bit_cast(T, (uint16_t)(v[i][j >> 1] >> ((j & 1) * 16)));
-      km = fmaxf(km, magnitude(kx[j]));
-      vm = fmaxf(vm, magnitude(vx[j]));
-    }
-#pragma unroll
-    for (int o = LR / 2; o > 0; o >>= 1) {
-      km = fmaxf(km, __shfl_xor(km, o, MSA_WAVE));
-      vm = fmaxf(vm, __shfl_xor(vm, o, MSA_WAVE));
-    }
-    const int ke = exponent_of<F>(fminf(km, cap)), ve = exponent_of<F>(fminf(vm, cap));
-    const float ks = inverse_power(ke), vs = inverse_power(ve);
-    auto held = [&](float x) { return x > cap ? cap : x < -cap ? -cap : x; };
-    auto four = [&](const float* x, float f) {
-      return code2<F>(held(x[0]) * f, held(x[1]) * f) | code2<F>(held(x[2]) * f, held(x[3]) * f) << 16;
-    };
+    int ke, ve;
+    const pg_u2 kc = quantise8<DT, F, LR>(k[i], ke), vc = quantise8<DT, F, LR>(v[i], ve);
     if (lane * 8 < HD) {
-      if (pg >= 0) *(pg_u2*)((uint8_t*)a.c.k_pages + place * HD + lane * 8) = pg_u2{four(kx, ks), four(kx + 4, ks)};
-      *(uint32_t*)(lds + at * STRIDE + lane * 8) = four(vx, vs);
-      *(uint32_t*)(lds + at * STRIDE + lane * 8 + 4) = four(vx + 4, vs);
+      if (pg >= 0) *(pg_u2*)((uint8_t*)a.c.k_pages + place * HD + lane * 8) = kc;
+      *(uint32_t*)(lds + at * STRIDE + lane * 8) = vc[0];
+      *(uint32_t*)(lds + at * STRIDE + lane * 8 + 4) = vc[1];
     }
     if (pg >= 0 && lane == 0) a.c.k_exp[place] = (int8_t)ke, a.c.v_exp[place] = (int8_t)ve;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < HD * NG; i += 256) {
-    const int d = i / NG, g = i % NG, p = b.first + g * G;
+  // a thread turns a word (W dimensions) of G positions into 16 bytes of each dimension
+  constexpr int W = 4 / ES;
+  for (int i = threadIdx.x; i < HD / W * NG; i += 256) {
+    const int d = i / NG * W, g = i % NG, p = b.first + g * G;
     if (p + G <= b.begin || p >= b.end) continue;
     const int pg = page_of(a, s, p);
     if (pg < 0) continue;
     char* to = (char*)a.c.v_pages + ((((int64_t)pg * a.c.kv_heads + h) * HD + d) * page + (p & (page - 1))) * ES;
     const char* from = lds + g * G * STRIDE + d * ES;
     if (p >= b.begin && p + G <= b.end) {
-      pg_u4 w;
+      uint32_t w[G];
+      pg_u4 o[W];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (ES == 2) {
-          w[j] = *(const uint16_t*)(from + 2 * j * STRIDE) | (uint32_t)*(const uint16_t*)(from + (2 * j + 1) * STRIDE) << 16;
-        } else {
-          w[j] = 0;
+      for (int j = 0; j < G; ++j) w[j] = *(const uint32_t*)(from + j * STRIDE);
+      if (ES == 2) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) w[j] |= (uint32_t)*(const uint8_t*)(from + (4 * j + e) * STRIDE) << (8 * e);
+        for (int j = 0; j < 4; ++j) {
+          o[0][j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x05040100u);
+          o[1][j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x07060302u);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t *x = w + 4 * j, lo = __builtin_amdgcn_perm(x[1], x[0], 0x05010400u), hi = __builtin_amdgcn_perm(x[1], x[0], 0x07030602u),
+                         lo2 = __builtin_amdgcn_perm(x[3], x[2], 0x05010400u), hi2 = __builtin_amdgcn_perm(x[3], x[2], 0x07030602u);
+          o[0][j] = __builtin_amdgcn_perm(lo2, lo, 0x05040100u);
+          o[1 % W][j] = __builtin_amdgcn_perm(lo2, lo, 0x07060302u);
+          o[2 % W][j] = __builtin_amdgcn_perm(hi2, hi, 0x05040100u);
+          o[3 % W][j] = __builtin_amdgcn_perm(hi2, hi, 0x07060302u);
         }
       }
-      *(pg_u4*)to = w;
+#pragma unroll
+      for (int k = 0; k < W; ++k) *(pg_u4*)(to + (int64_t)k * page * ES) = o[k];
     } else {  // positions beside the new ones stay as they are
-      for (int j = max(b.begin - p, 0); j < min(b.end - p, G); ++j) {
-        if (ES == 2) ((uint16_t*)to)[j] = *(const uint16_t*)(from + j * STRIDE);
-        else ((uint8_t*)to)[j] = *(const uint8_t*)(from + j * STRIDE);
-      }
+      for (int j = max(b.begin - p, 0); j < min(b.end - p, G); ++j)
+        for (int k = 0; k < W; ++k) {
+          if (ES == 2) ((uint16_t*)to)[k * page + j] = *(const uint16_t*)(from + j * STRIDE + k * 2);
+          else ((uint8_t*)to)[k * page + j] = *(const uint8_t*)(from + j * STRIDE + k);
+        }
     }
   }
 }
@@ -286,9 +344,11 @@ __global__ __launch_bounds__(256) void read_block_kernel(PagedRows a, int blocks
   constexpr int ES = F < PG_E4M3 ? 2 : 1, LR = row_lanes<HD>(), RP = 256 / LR, N = PB / RP;
   constexpr int STRIDE = HD * ES + 4, G = 16 / ES, NG = PB / G, NV = (HD * NG + 255) / 256;
   __shared__ __attribute__((aligned(16))) char lds[PB * STRIDE];
-  const int s = blockIdx.x / blocks, h = blockIdx.y, lane = threadIdx.x % LR, r0 = threadIdx.x / LR;
+  // (the heads of a block next to one another: their pieces of a row are)
+  const int sb = blockIdx.x / a.c.kv_heads, h = blockIdx.x - sb * a.c.kv_heads, s = sb / blocks;
+  const int lane = threadIdx.x % LR, r0 = threadIdx.x / LR;
   Block b;
-  if (!block_of(a, s, blockIdx.x - s * blocks, b)) return;
+  if (!block_of(a, s, sb - s * blocks, b)) return;
   const int page = 1 << a.page_log2;
   // 8 codes (or two words more of 16 bits) times 2^e as 16 bytes of T
   auto rows_of = [](pg_u4 w, int e) {
@@ -368,7 +428,7 @@ void launch_rows_hd(const PagedRows& a, bool append, hipStream_t s) {
     return;
   }
   const int blocks = (a.b.max_count + PB - 2) / PB + 1;  // that max_count positions can meet
-  const dim3 grid((unsigned)(a.b.nseq * blocks), (unsigned)a.c.kv_heads);
+  const dim3 grid((unsigned)((int64_t)a.b.nseq * blocks * a.c.kv_heads));
   if (append) hipLaunchKernelGGL((append_block_kernel<DT, F, HD>), grid, dim3(256), 0, s, a, blocks);
   else hipLaunchKernelGGL((read_block_kernel<DT, F, HD>), grid, dim3(256), 0, s, a, blocks);
 }
@@ -403,7 +463,7 @@ int check_rows(const msa_paged_cache* c, const msa_paged_batch* b, const void* k
   MSA_REQUIRE(k && v, MSA_ERR_INVALID_ARG, "%s: null pointer", who);
   MSA_REQUIRE(((uintptr_t)k | (uintptr_t)v) % 16 == 0, MSA_ERR_INVALID_ARG, "%s: keys and values must be 16-byte aligned", who);
   const int64_t n = (int64_t)c->kv_heads * c->hd;
-  MSA_REQUIRE((int64_t)b->nseq * ((b->max_count + 62) / 64 + 1) <= INT32_MAX, MSA_ERR_INVALID_ARG, "%s: too many rows for one call", who);
+  MSA_REQUIRE((int64_t)b->nseq * (((int64_t)b->max_count + 62) / 64 + 1) * c->kv_heads <= INT32_MAX, MSA_ERR_INVALID_ARG, "%s: too many rows for one call", who);
   MSA_REQUIRE(ldk >= n && ldv >= n && ldk % 8 == 0 && ldv % 8 == 0, MSA_ERR_INVALID_ARG,
               "%s: row strides must be multiples of 8 of at least kv_heads * hd", who);
   return MSA_OK;
