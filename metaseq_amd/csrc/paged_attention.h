@@ -635,13 +635,27 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
   // ---- tiles.  (The table is read through the scalar cache: a vector load would be waited for together with all the
   // loads to LDS in front of it) ----
   const pg_uniform_i32* table = (const pg_uniform_i32*)(uintptr_t)(a.table + (int64_t)s * a.table_stride);
-  // page of the sixteen keys g16 of tile i, -1 where there is none
-  auto look = [&](int i, int g16) {
-    const int block = (tiles.tile(i) * PT_BN + g16 * 16) >> a.page_log2;
-    const int pg = table[min(block, a.blocks - 1)];
-    return block < a.blocks && (unsigned)pg < (unsigned)a.pages ? pg : -1;
+  // entries of the pages of tile i's four groups of sixteen keys (one entry of pages of 64 and more), to be checked when they
+  // are used: a check here would wait for them
+  const bool large = a.page_log2 >= 6;
+  auto entries = [&](int i) {
+    const int key0 = tiles.tile(min(i, it_end - 1)) * PT_BN, last = a.blocks - 1;
+    PtPages e;
+    e.a = table[min(key0 >> a.page_log2, last)];
+    e.b = e.c = e.d = e.a;
+    if (!large) {
+      e.b = table[min((key0 + 16) >> a.page_log2, last)];
+      e.c = table[min((key0 + 32) >> a.page_log2, last)];
+      e.d = table[min((key0 + 48) >> a.page_log2, last)];
+    }
+    return e;
   };
-  const int64_t unit = (int64_t)page * HD * ES;
+  auto checked = [&](PtPages e, int i) {
+    const int key0 = tiles.tile(i) * PT_BN;
+    auto one = [&](int pg, int key) { return (key >> a.page_log2) < a.blocks && (unsigned)pg < (unsigned)a.pages ? pg : -1; };
+    return PtPages{one(e.a, key0), one(e.b, key0 + 16), one(e.c, key0 + 32), one(e.d, key0 + 48)};
+  };
+  const int64_t unit = (int64_t)page * HD * ES, page_bytes = unit * a.kv_heads;  // of a page and head, of a page
   const uint32_t lds0 = (uint32_t)(uintptr_t)(pt_lds_void*)lds;
   // 16 bits.  Keys: the sixteen of this wave, which are of one page, fill its sixteen rows of the tile.  Values: every
   // fourth group of eight rows (dimensions) is this wave's; a lane has the same chunk (eight keys) in all of them.
@@ -655,11 +669,11 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
       koff[u] = row * ROWB + pt_chunk_at<CH>(at % CH, row) * 16;
     }
   }
+  const char *k_head = (const char*)a.k_pages + h * unit, *v_lane = (const char*)a.v_pages + h * unit + vrow * page * 2;
   auto issue = [&](int i, int slot, PtPages pg) {
     const int key0 = tiles.tile(i) * PT_BN, in = page - 1;
     {
-      const int p = pg.of(wave);
-      const char* from = (const char*)a.k_pages + ((int64_t)max(p, 0) * a.kv_heads + h) * unit + (int64_t)((key0 + wave * 16) & in) * ROWB;
+      const char* from = k_head + max(pg.of(wave), 0) * page_bytes + ((key0 + wave * 16) & in) * ROWB;
 #pragma unroll
       for (int u = 0; u < KI; ++u) {
         const uint32_t la = lds0 + slot * TILEB + wave * 16 * ROWB + u * 1024;
@@ -667,9 +681,7 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
           asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(koff[u]), "s"(pt_uniform(from)), "s"(la) : "memory");
       }
     }
-    auto at = [&](int k) { return ((int64_t)max(pg.of(k), 0) * a.kv_heads + h) * unit + ((key0 + k * 16) & in) * 2; };
-    const int64_t at0 = at(0), at1 = at(1), at2 = at(2), at3 = at(3);
-    const char* from = (const char*)a.v_pages + (vc < 4 ? (vc < 2 ? at0 : at1) : (vc < 6 ? at2 : at3)) + (vc & 1) * 16 + vrow * page * 2;
+    const char* from = v_lane + max(pg.of(vc >> 1), 0) * page_bytes + ((key0 + vc * 8) & in) * 2;
 #pragma unroll
     for (int u = 0; u < VI; ++u) {
       const uint32_t la = lds0 + (2 + slot) * TILEB + (u * 4 + wave) * 1024;
@@ -764,14 +776,10 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
   for (int d = 0; d < DBLK; ++d) o[d] = zero16;
   float m = -INFINITY, l = 0.f;
   int E = -127, ek = 0, ev = -127;  // what the accumulators are relative to, and this tile's keys and values
-  auto look4 = [&](int i) {
-    const int j = min(i, it_end - 1);
-    return PtPages{look(j, 0), look(j, 1), look(j, 2), look(j, 3)};
-  };
-  PtPages pg = {-1, -1, -1, -1}, next = pg;  // this tile's and the next one's
+  PtPages pg = {-1, -1, -1, -1}, next = pg;  // this tile's, and entries of the next one's
   if (it0 < it_end) {
-    pg = look4(it0);
-    next = look4(it0 + 1);
+    pg = checked(entries(it0), it0);
+    next = entries(it0 + 1);
     if (B8) {
       fetch(it0, pg);
       stage(it0, 0, pg, ek, ev);
@@ -779,18 +787,20 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
       issue(it0, 0, pg);
     }
   }
+  // (the queries have arrived from here on: the compiler, which does not count the loads to LDS, would wait for them in the
+  // loop, and with them for the tile just requested)
+#pragma unroll
+  for (int ks = 0; ks < KSTEPS; ++ks) asm volatile("" : "+v"(qf[ks]));
   for (int i = it0; i < it_end; ++i) {
     const int slot = (i - it0) & 1;
     const int here = (pg.a >= 0 ? 1 : 0) | (pg.b >= 0 ? 2 : 0) | (pg.c >= 0 ? 4 : 0) | (pg.d >= 0 ? 8 : 0);
     if (!B8) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();  // the tile is complete, and the other slots are free
     if (i + 1 < it_end) {
-      if (B8) fetch(i + 1, next);
-      else issue(i + 1, slot ^ 1, next);
+      pg = checked(next, i + 1);
+      if (B8) fetch(i + 1, pg);
+      else issue(i + 1, slot ^ 1, pg);
     }
-    pg = next;
-    next = look4(i + 2);
-
     const char* kt = lds + slot * TILEB;
     char* vt = lds + (2 + slot) * TILEB;
     const int key0 = tiles.tile(i) * PT_BN;
@@ -800,19 +810,22 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
     // infinity is NaN), so it is added to those and left out of the product.
     bool odd = false;
     if (F != PG_I8 && !(key0 + PT_BN - 1 <= g_lo && (a.window <= 0 || key0 > g_hi - a.window || key0 + PT_BN <= a.sinks) && here == 15)) {
+      typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+      u16x2 most = {0, 0};
 #pragma unroll 1
       for (int at = threadIdx.x; at < HD * 8; at += PT_THREADS) {
         const int key = key0 + pt_chunk_at<8>(at & 7, at >> 3) * 8;
-        const bool there = (here >> ((key - key0) >> 4)) & 1;
-        const uint32_t seen = there ? pa_seen<8>(key, g_lo, g_hi, a.window, a.sinks) : 0;
+        const uint32_t seen = (here >> ((key - key0) >> 4)) & 1 ? pa_seen<8>(key, g_lo, g_hi, a.window, a.sinks) : 0;
         pg_u4 v = *(pg_u4*)(vt + at * 16);
+        if (seen != 255) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          v[k] = pa_keep<G>(v[k], seen >> (2 * k));
-          odd |= pa_not_finite<G>(v[k], 0) != 0;
+          for (int k = 0; k < 4; ++k) v[k] = pa_keep<G>(v[k], seen >> (2 * k));
+          *(pg_u4*)(vt + at * 16) = v;
         }
-        if (seen != 255) *(pg_u4*)(vt + at * 16) = v;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, v[k] & 0x7fff7fffu));
       }
+      odd = max(most[0], most[1]) >= (G == PG_BF16 ? 0x7f80 : 0x7c00);
       odd = __syncthreads_or(odd);
     }
     // (a wave whose rows see nothing of the tile has nothing to do)
@@ -865,25 +878,23 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
       }
       const float off = (m == -INFINITY ? 0.f : m) - SHIFT;
       pg_u4 p[4];  // steps of sixteen keys of the product with V
-      float sum[2] = {0.f, 0.f};
+      float sum[2] = {0.f, 0.f};  // of the probabilities as they are rounded
 #pragma unroll
       for (int st = 0; st < 4; ++st) {
         float e[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[st * 8 + j], c, -off));
-          sum[j & 1] += e[j];
-        }
-        if (F == PG_BF16) {
-          bf16x8_t w;
+        for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[st * 8 + j], c, -off));
 #pragma unroll
-          for (int j = 0; j < 8; ++j) w[j] = (bf16_t)e[j];
-          p[st] = __builtin_bit_cast(pg_u4, w);
-        } else {
-          half8_t w;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) w[j] = (half_t)e[j];
-          p[st] = __builtin_bit_cast(pg_u4, w);
+        for (int j = 0; j < 4; ++j) {
+          if (F == PG_BF16) {
+            const bf16x2_t w = {(bf16_t)e[2 * j], (bf16_t)e[2 * j + 1]}, one = {(bf16_t)1.f, (bf16_t)1.f};
+            sum[j & 1] = __builtin_amdgcn_fdot2_f32_bf16(w, one, sum[j & 1], false);
+            p[st][j] = __builtin_bit_cast(uint32_t, w);
+          } else {
+            const half2_t w = {(half_t)e[2 * j], (half_t)e[2 * j + 1]}, one = {(half_t)1.f, (half_t)1.f};
+            sum[j & 1] = __builtin_amdgcn_fdot2(w, one, sum[j & 1], false);
+            p[st][j] = __builtin_bit_cast(uint32_t, w);
+          }
         }
       }
       l += sum[0] + sum[1];
@@ -923,6 +934,7 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
     if (whole) attend(std::false_type{});
     else if (!none) attend(std::true_type{});
     if (B8 && i + 1 < it_end) stage(i + 1, slot ^ 1, pg, ek, ev);
+    next = entries(i + 2);
   }
 
   // ---- O^T: row n32, dimensions 32 db + 8 blk + 4 hl + r ----
