@@ -37,7 +37,7 @@ typedef struct {
  * stay as they were); seq_pos [nseq]: position of its first row (negative: the sequence sits this call out, its
  * outputs stay as they were).  Position p of sequence s is in page table[s * table_stride + p / page]; positions
  * whose entry is outside 0 .. pages - 1, or beyond the `blocks` entries of a sequence, are nowhere: they are not written,
- * read back as zeros and seen by no row.  max_count: no sequence has more rows (those that it has beyond are left
+ * read back as zeros and seen by no row.  A table names at most 2^30 positions.  max_count: no sequence has more rows (those that it has beyond are left
  * alone); min_count: no sequence that has rows has fewer (0: not known); key_bound: no row's position reaches it (a hint: how keys are split follows from it, results up to
  * rounding do not). */
 typedef struct {

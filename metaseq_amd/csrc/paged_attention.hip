@@ -158,9 +158,11 @@ extern "C" int msa_paged_attention(const msa_paged_cache* c, const msa_paged_bat
   const int64_t units = (int64_t)b->nseq * c->kv_heads;
   MSA_REQUIRE((int64_t)b->nseq * PA_FEW <= INT32_MAX && units * p.row_blocks <= INT32_MAX && (units + 7) * p.tile_blocks * p.tile_splits <= INT32_MAX,
               MSA_ERR_INVALID_ARG, "msa_paged_attention: too many rows for one call");
+  // (positions are below 2^30; a window that holds them all is none)
+  const int window = a->window < (int64_t)b->blocks * c->page ? a->window : 0;
   PagedAttention k = {a->q, c->k_pages, c->v_pages, c->k_exp, c->v_exp, b->seq_start, b->seq_pos, b->table, a->ldq, a->ldo,
                       b->table_stride, a->out, (float*)a->workspace, b->M, b->nseq, a->heads, c->kv_heads, c->pages,
-                      paged_log2(c->page), b->blocks, a->out_mb, a->window, a->sinks, 1, 1,
+                      paged_log2(c->page), b->blocks, a->out_mb, window, a->sinks, 1, 1,
                       c->dtype == MSA_BF16, b->max_count, PA_FEW, p.grouped, a->scale};
   hipStream_t s = (hipStream_t)stream;
   const int format = paged_format(*c);

@@ -456,10 +456,12 @@ void launch_rows(const PagedRows& a, bool append, hipStream_t s) {
   return launch_rows_format<MSA_BF16, PG_I8>(a, append, s);
 }
 
+bool nothing(const msa_paged_batch* b) { return b->M == 0 || b->nseq == 0 || b->max_count == 0; }
+
 int check_rows(const msa_paged_cache* c, const msa_paged_batch* b, const void* k, int64_t ldk, const void* v, int64_t ldv,
                const char* who) {
   const int rc = msa_paged_check(c, b, who);
-  if (rc) return rc;
+  if (rc || nothing(b)) return rc;  // (rows that do not exist need no memory)
   MSA_REQUIRE(k && v, MSA_ERR_INVALID_ARG, "%s: null pointer", who);
   MSA_REQUIRE(((uintptr_t)k | (uintptr_t)v) % 16 == 0, MSA_ERR_INVALID_ARG, "%s: keys and values must be 16-byte aligned", who);
   const int64_t n = (int64_t)c->kv_heads * c->hd;
@@ -488,8 +490,8 @@ int msa_paged_check(const msa_paged_cache* c, const msa_paged_batch* b, const ch
   MSA_REQUIRE(b->M >= 0 && b->nseq >= 0 && b->nseq <= (1 << 20) && b->max_count >= 0 && b->key_bound >= 0, MSA_ERR_INVALID_ARG,
               "%s: negative sizes, or more than 2^20 sequences", who);
   MSA_REQUIRE(b->min_count >= 0 && b->min_count <= b->max_count, MSA_ERR_INVALID_ARG, "%s: min_count must be 0 .. max_count", who);
-  MSA_REQUIRE(b->blocks >= 1 && b->table_stride >= b->blocks && (int64_t)b->blocks * c->page <= INT32_MAX,
-              MSA_ERR_INVALID_ARG, "%s: blocks must be positive, at most table_stride and 2^31 positions", who);
+  MSA_REQUIRE(b->blocks >= 1 && b->table_stride >= b->blocks && (int64_t)b->blocks * c->page <= 1 << 30,
+              MSA_ERR_INVALID_ARG, "%s: blocks must be positive, at most table_stride and 2^30 positions", who);
   MSA_REQUIRE(b->nseq == 0 || (b->seq_start && b->seq_pos && b->table), MSA_ERR_INVALID_ARG, "%s: null pointer", who);
   return MSA_OK;
 }
@@ -497,8 +499,7 @@ int msa_paged_check(const msa_paged_cache* c, const msa_paged_batch* b, const ch
 extern "C" int msa_paged_append(const msa_paged_cache* c, const msa_paged_batch* b, const void* k, int64_t ldk, const void* v,
                                 int64_t ldv, void* stream) {
   const int rc = check_rows(c, b, k, ldk, v, ldv, "msa_paged_append");
-  if (rc) return rc;
-  if (b->M == 0 || b->nseq == 0 || b->max_count == 0) return MSA_OK;
+  if (rc || nothing(b)) return rc;
   hipStream_t s = (hipStream_t)stream;
   const PagedRows a = {*c, *b, k, v, nullptr, nullptr, ldk, ldv, paged_log2(c->page)};
   launch_rows(a, true, s);
@@ -509,8 +510,7 @@ extern "C" int msa_paged_append(const msa_paged_cache* c, const msa_paged_batch*
 extern "C" int msa_paged_read(const msa_paged_cache* c, const msa_paged_batch* b, void* k, int64_t ldk, void* v, int64_t ldv,
                               void* stream) {
   const int rc = check_rows(c, b, k, ldk, v, ldv, "msa_paged_read");
-  if (rc) return rc;
-  if (b->M == 0 || b->nseq == 0 || b->max_count == 0) return MSA_OK;
+  if (rc || nothing(b)) return rc;
   hipStream_t s = (hipStream_t)stream;
   const PagedRows a = {*c, *b, nullptr, nullptr, k, v, ldk, ldv, paged_log2(c->page)};
   launch_rows(a, false, s);

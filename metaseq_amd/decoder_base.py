@@ -169,6 +169,8 @@ class IncrementalDecoder(nn.Module):
     def release_slot(self, cache, slot: int):
         # a fill kernel on a one-element view: ``lens[slot] = -1`` copies a host scalar to the
         # device and makes the caller wait for the work queued ahead of it
+        if hasattr(cache, "release_row"):
+            cache.release_row(slot)
         cache.lens[slot:slot + 1].fill_(-1)
 
     def _sample_rows(self, lib, logits, sampled, banned, stop, finished, eos, tok_out, score_out):

@@ -223,3 +223,154 @@ class PagedCache:
             a.workspace, a.workspace_bytes = ws.data_ptr(), need
         self._run(self._lib.msa_paged_attention, c, batch.by_ref, ref)
         return out
+
+
+class PagedSlots:
+    """The cache of a decoder's slots in pages: one ``PagedCache`` per layer, one table for all of them, and the
+    pages that no slot holds (``TransformerDecoder.new_paged_cache``).  It takes the place of a slot ``KVCache``: a
+    slot is filled by prefills or ``extend``, advanced by decode steps, copied and released.
+
+    A slot takes pages as it grows.  Copies share the full pages of what they copy (``refs`` counts the holders).
+    With ``window``, attention is over the last ``window`` positions and the first ``sinks``, and a page that no
+    position to come can see is given back by the next ``extend``.  ``lens``: positions each slot holds (int32 on the
+    device, negative: empty); ``host_lens``: the same on the host, except that decode steps count every slot of
+    ``stale`` as having taken part, which only the device knows."""
+
+    has_pads = False
+    ragged = True
+
+    def __init__(self, n_layers, slots, capacity, kv_heads, head_dim, pages, page, dtype, window, sinks, device):
+        blocks = -(-capacity // page)
+        self.batch, self.capacity, self.page, self.device = int(slots), int(capacity), int(page), device
+        self.window, self.sinks = int(window), int(sinks)
+        if self.window < 0 or self.sinks < 0:
+            raise ValueError("window and sinks must not be negative")
+        self.layers = [PagedCache.empty(pages, kv_heads, head_dim, page, dtype, device) for _ in range(n_layers)]
+        self.lens = torch.full((self.batch,), -1, dtype=torch.int32, device=device)
+        self.host_lens = [-1] * self.batch
+        self.table = torch.full((self.batch, blocks), -1, dtype=torch.int32, device=device)
+        self.host_table = torch.full((self.batch, blocks), -1, dtype=torch.int32)
+        self.refs = [0] * pages
+        self.free = list(range(pages - 1, -1, -1))
+        self._passed = [0] * self.batch   # blocks below, behind those of the first positions, have been given back
+        self.stale = set()
+
+    def _page(self):
+        if not self.free:
+            raise ValueError("all %d pages are held" % len(self.refs))
+        at = self.free.pop()
+        self.refs[at] = 1
+        return at
+
+    def _drop(self, at):
+        self.refs[at] -= 1
+        if self.refs[at] == 0:
+            self.free.append(at)
+
+    def reserve(self, wanted):
+        """Pages for the positions [pos, pos + n) of every (slot, pos, n); all of them or, with ValueError, none."""
+        if any(pos + n > self.capacity for _, pos, n in wanted):
+            raise ValueError("a slot would hold more than %d positions" % self.capacity)
+        new = [(s, b) for s, pos, n in wanted for b in range(pos // self.page, -(-(pos + n) // self.page))
+               if int(self.host_table[s, b]) < 0]
+        # a page that others hold too is not written to: whose next position lies in one gets a copy, but for the last
+        copies, left = [], {}
+        for s, pos, n in wanted:
+            at = int(self.host_table[s, pos // self.page]) if n and pos % self.page else -1
+            if at >= 0 and left.setdefault(at, self.refs[at]) > 1:
+                left[at] -= 1
+                copies.append((s, pos // self.page))
+        if len(new) + len(copies) > len(self.free):
+            raise ValueError("%d pages are needed, %d are free" % (len(new) + len(copies), len(self.free)))
+        for s, b in new:
+            self.host_table[s, b] = self._page()
+        for s, b in copies:
+            old = int(self.host_table[s, b])
+            self.host_table[s, b] = self._page()
+            self._copy_page(old, int(self.host_table[s, b]))
+            self._drop(old)
+        if new or copies:
+            self._upload()
+
+    def _copy_page(self, src, dst):
+        for layer in self.layers:
+            for t in (layer.k_pages, layer.v_pages, layer.k_exp, layer.v_exp):
+                if t is not None:
+                    t[dst].view(torch.uint8).copy_(t[src].view(torch.uint8))
+
+    def _upload(self):
+        # (a copy in pinned memory of its own: the host table changes while the transfer is on its way)
+        t = self.host_table.pin_memory() if self.table.is_cuda else self.host_table
+        self.table.copy_(t, non_blocking=True)
+
+    def exact_lens(self, slots):
+        """Makes ``host_lens`` exact where decode steps may have left one of ``slots`` out (waits for the device)."""
+        if not self.stale.isdisjoint(slots):
+            lens = self.lens.tolist()
+            for s in self.stale:
+                self.host_lens[s] = lens[s]
+            self.stale.clear()
+
+    def holds(self, slot, n):
+        """``slot`` has exactly ``n`` positions from here on; pages behind the window go back."""
+        self.host_lens[slot] = n
+        self.stale.discard(slot)
+        if self.window:
+            first = max(-(-self.sinks // self.page), self._passed[slot])
+            past = max(first, (n - self.window + 1) // self.page)   # blocks below hold positions <= n - window only
+            for b in range(first, past):
+                if int(self.host_table[slot, b]) >= 0:
+                    self._drop(int(self.host_table[slot, b]))
+                    self.host_table[slot, b] = -1
+            self._passed[slot] = past
+
+    def release_row(self, slot):
+        for b in range(self.host_table.shape[1]):
+            if int(self.host_table[slot, b]) >= 0:
+                self._drop(int(self.host_table[slot, b]))
+        self.host_table[slot].fill_(-1)
+        self.host_lens[slot], self._passed[slot] = -1, 0
+        self.stale.discard(slot)
+
+    def copy_row(self, src, dst, n):
+        """Slot ``dst`` becomes slot ``src``, which holds ``n`` positions: it shares src's pages."""
+        if src == dst:
+            return
+        self.release_row(dst)
+        for b in range(-(-n // self.page)):
+            at = int(self.host_table[src, b])
+            if at >= 0:
+                self.refs[at] += 1
+                self.host_table[dst, b] = at
+        self.host_lens[dst], self._passed[dst] = n, self._passed[src]
+        self._upload()
+
+    def bytes(self):
+        return sum(layer.bytes() for layer in self.layers)
+
+
+class PagedRows:
+    """One step's rows through a decoder's layers (``PagedSlots``): ``attend(i, ...)`` stores layer i's new keys and values
+    and attends them.  Batch, work buffers and arguments are the same for all layers."""
+
+    def __init__(self, lib, slots, batch, heads, head_dim, device):
+        self.slots, self.batch, self.heads, self.layer = slots, batch, heads, 0
+        D = heads * head_dim
+        self.qkv = torch.empty(batch.rows, 3 * D, dtype=torch.float16, device=device)
+        self.D = D
+        first = slots.layers[0]
+        self.args = _capi.PagedAttentionArgs(heads, self.qkv.data_ptr() + 4 * D, 3 * D, None, D, 0, slots.window,
+                                             slots.sinks, 1.0 / math.sqrt(head_dim), None, 0)
+        need = lib.msa_paged_attention_workspace_bytes(first._of(torch.float16), batch.by_ref, ctypes.byref(self.args))
+        if need < 0:
+            _capi.check(need, lib)
+        self.workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=device)
+        self.args.workspace, self.args.workspace_bytes = self.workspace.data_ptr(), need
+
+    def attend(self, lib, stream, out, out_mb):
+        """Layer ``self.layer``: ``self.qkv`` holds the rows' keys, values and queries; ``out`` row-major, or packed
+        with ``out_mb`` row blocks."""
+        c, k = self.slots.layers[self.layer]._of(torch.float16), self.qkv.data_ptr()
+        _capi.check(lib.msa_paged_append(c, self.batch.by_ref, k, 3 * self.D, k + 2 * self.D, 3 * self.D, stream), lib)
+        self.args.out, self.args.out_mb = out.data_ptr(), out_mb
+        _capi.check(lib.msa_paged_attention(c, self.batch.by_ref, ctypes.byref(self.args), stream), lib)

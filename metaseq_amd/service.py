@@ -403,11 +403,14 @@ class ContinuousBatcher(_Front):
     to that many steps while rows are decoding, for company.  With the default (1, 0) every
     request is prefilled alone and its result does not depend on its neighbours to the last
     bit; a shared prefill runs on other tile shapes, so results can then differ in the last bit
-    of a logit, as they do between batches of the reference's own service."""
+    of a logit, as they do between batches of the reference's own service.
+
+    ``cache_args``: keyword arguments of the decoder's ``new_paged_cache`` (``dtype=torch.int8`` keeps keys and
+    values in 8 bits, ``page``, ``window``, ``sinks``): the slots then live in pages."""
 
     def __init__(self, interface, slots: int = 32, capacity: int = MAX_SEQ_LEN,
                  idle_ms: float = 2.0, noise_fn=None, patience: int = 64,
-                 prefill_batch: int = 1, prefill_wait: int = 0):
+                 prefill_batch: int = 1, prefill_wait: int = 0, cache_args: Optional[dict] = None):
         super().__init__(idle_ms / 1000.0)
         import torch
 
@@ -422,6 +425,7 @@ class ContinuousBatcher(_Front):
         self.batch = SlotBatch(slots, capacity)
         self.backlog = Backlog()
         self.cache = None  # allocated with the first request
+        self.cache_args = cache_args
         self._stop: tuple = ()  # stop ids of the running batch
         self.noise_fn, self.patience = noise_fn, int(patience)
         self.prefill_batch, self.prefill_wait = max(1, int(prefill_batch)), int(prefill_wait)
@@ -671,8 +675,9 @@ class ContinuousBatcher(_Front):
         values are copied to its replicas' slots and each replica's first token is chosen from
         the prompt's last position.  An error is the answer of every request it concerns."""
         if self.cache is None:
-            self.cache = self.decoder.new_slot_cache(len(self.batch.rows), self.batch.capacity,
-                                                     self.device)
+            new = self.decoder.new_slot_cache if self.cache_args is None else self.decoder.new_paged_cache
+            self.cache = new(len(self.batch.rows), self.batch.capacity, device=self.device,
+                             **(self.cache_args or {}))
         torch = self._torch
         total = sum(len(slots) for slots, _ in items)
         tok_all = torch.zeros(total, dtype=torch.long, device=self.device)

@@ -22,6 +22,7 @@ from .checkpoint_utils import quantize_rows
 from .config import OPTConfig
 from .decoder_base import IncrementalDecoder, upload
 from .kv_cache import KVCache
+from .paged_cache import PagedRows, PagedSlots
 
 
 class _Affine(nn.Module):
@@ -759,7 +760,7 @@ class TransformerDecoder(IncrementalDecoder):
         return features, packed, (B, T), {"inner_states": inner_states}
 
     def _rows_core(self, lib, stream, tokens, B, n, T, S0, kv, mask, token_embeddings=None,
-                   len_dev=None, step_len=None, prompts=None, want_packed=False):
+                   len_dev=None, step_len=None, prompts=None, want_packed=False, paged=None):
         """Prefill (or a decode batch above 128 rows): the last T columns of ``tokens[B, n]``
         through embedding, L layers and the final LayerNorm on row-major activations and the
         tiled MFMA kernels, keys and values written at positions S0 .. S0 + T - 1 of ``kv``
@@ -770,7 +771,8 @@ class TransformerDecoder(IncrementalDecoder):
         step used (-1 for the rows that sat it out).  With ``prompts`` (_Prompts; S0 == 0) the
         pads are dropped behind the embedding: everything runs over the prompts' own rows, one
         after the other, and their keys and values go to the cache rows they name.  ``want_packed``
-        (at most 64 rows): the features leave in the packed activation layout."""
+        (at most 64 rows): the features leave in the packed activation layout.  ``paged`` (PagedRows, T == 1,
+        ``kv`` None): keys and values of the B rows live in pages."""
         cfg = self.cfg
         D = cfg.decoder_embed_dim
         dev = tokens.device
@@ -799,8 +801,11 @@ class TransformerDecoder(IncrementalDecoder):
             last = i + 1 == len(self.layers)
             after = (None if self.layer_probe is not None else self.layer_norm if last
                      else self.layers[i + 1].self_attn_layer_norm)
-            self._rows_layer(lib, stream, layer, x, work, B, T, S0, kv.k(i), kv.v(i),
-                             kv.capacity, mask, len_dev, prompts, after, last and not want_packed)
+            if paged is not None:
+                paged.layer = i
+            where = (kv.k(i), kv.v(i), kv.capacity) if paged is None else (None, None, 0)
+            self._rows_layer(lib, stream, layer, x, work, B, T, S0, *where, mask, len_dev, prompts, after,
+                             last and not want_packed, paged)
             if self.layer_probe is not None:
                 self.layer_probe(i, x)
         if self.return_inner_states:
@@ -868,7 +873,7 @@ class TransformerDecoder(IncrementalDecoder):
                                     ptr(o), B, H, hd, T, S0, cap, 0, ptr(len_dev), stream))
 
     def _rows_layer(self, lib, stream, layer, x, work, B, T, S0, kc, vc, cap, mask, len_dev=None,
-                    prompts=None, after=None, last=False):
+                    prompts=None, after=None, last=False, paged=None):
         """One layer over B * T row-major rows (transformer_decoder_layer.py:233-284): ``x`` is
         the residual stream, updated in place; keys and values of the T new positions of every
         row go to positions S0 .. S0 + T - 1 of ``kc`` / ``vc``.  Where fc2 runs as partial sums, the launch
@@ -880,13 +885,17 @@ class TransformerDecoder(IncrementalDecoder):
         M = B * T
         if M <= self.PACKED_MAX_ROWS:
             return self._rows_layer_short(lib, stream, layer, x, work, B, T, S0, kc, vc, cap, mask,
-                                          len_dev, prompts, after, last)
+                                          len_dev, prompts, after, last, paged)
         q, h, o, u = work["q"], work["h"], work["o"], work["u"]
         if not work["normed"]:
             self._layernorm(lib, stream, x, layer.self_attn_layer_norm, M, D, h)
-        self._qkv(lib, stream, h, layer.self_attn.qkv_proj, q, kc, vc, B, T, H, hd, S0, cap, D, 0,
-                  len_dev, prompts)
-        self._rows_attention(lib, stream, q, kc, vc, mask, o, B, H, hd, T, S0, cap, len_dev, prompts)
+        if paged is not None:
+            self._linear(lib, stream, h, layer.self_attn.qkv_proj, M, 3 * D, D, out=paged.qkv)
+            paged.attend(lib, stream, o, 0)
+        else:
+            self._qkv(lib, stream, h, layer.self_attn.qkv_proj, q, kc, vc, B, T, H, hd, S0, cap, D, 0,
+                      len_dev, prompts)
+            self._rows_attention(lib, stream, q, kc, vc, mask, o, B, H, hd, T, S0, cap, len_dev, prompts)
         # x = round(round(o Wo^T + bo) + x)   (transformer_decoder_layer.py:222-230)
         ln2 = layer.final_layer_norm
         if not self._linear_split(lib, stream, o, layer.self_attn.out_proj, x, work, M, D, D,
@@ -901,7 +910,7 @@ class TransformerDecoder(IncrementalDecoder):
         work["normed"] = work["normed"] and after is not None
 
     def _rows_layer_short(self, lib, stream, layer, x, work, B, T, S0, kc, vc, cap, mask,
-                          len_dev=None, prompts=None, after=None, last=False):
+                          len_dev=None, prompts=None, after=None, last=False, paged=None):
         """``_rows_layer`` for at most 128 rows (a short prompt): the layer's GEMM inputs are
         produced in the packed activation layout by the kernels in front of them, so that qkv,
         out_proj, fc1 and fc2 run on the packed kernels of the decode step (57 rows, OPT-6.7B
@@ -919,10 +928,15 @@ class TransformerDecoder(IncrementalDecoder):
         hp, op, up, S_o, S_f = (work[k] for k in ("hp", "op", "up", "S_o", "S_f"))
         if not work["normed"]:
             self._layernorm(lib, stream, x, layer.self_attn_layer_norm, M, D, hp, OUT)
-        self._qkv(lib, stream, hp, layer.self_attn.qkv_proj, q, kc, vc, B, T, H, hd, S0, cap, D, IN,
-                  len_dev, prompts)
+        if paged is not None:
+            self._linear(lib, stream, hp, layer.self_attn.qkv_proj, M, 3 * D, D, out=paged.qkv, flags=IN)
+        else:
+            self._qkv(lib, stream, hp, layer.self_attn.qkv_proj, q, kc, vc, B, T, H, hd, S0, cap, D, IN,
+                      len_dev, prompts)
         mask_stride = mask.stride(0) if mask is not None else 0
-        if prompts is not None:
+        if paged is not None:
+            paged.attend(lib, stream, op, self._packed_rows(M) // 16)
+        elif prompts is not None:
             check(lib.msa_attention_packed_f16(ptr(q), ptr(kc), ptr(vc), None, 0, ptr(op), ptr(prompts.start),
                                                ptr(prompts.slot), M, prompts.count, H, hd, prompts.longest, 0, cap,
                                                stream))
@@ -993,6 +1007,139 @@ class TransformerDecoder(IncrementalDecoder):
         cache.lens = torch.full((slots,), -1, dtype=torch.int32, device=dev)
         return cache
 
+    PORTION = 8192   # most tokens of one pass of ``extend``
+
+    def new_paged_cache(self, slots: int, capacity: int, pages=None, page: int = 64, dtype=torch.float16,
+                        window: int = 0, sinks: int = 0, device=None) -> PagedSlots:
+        """An empty cache of ``slots`` rows (at most 256) of up to ``capacity`` positions each that keeps keys and
+        values in ``pages`` pages of ``page`` positions (default: enough for every slot at its capacity), as fp16 or
+        in 8 bits (``dtype`` float8_e4m3fn or int8).  ``window``: attention over the last ``window`` positions and
+        the first ``sinks`` only.  For ``extend`` and the slot interface."""
+        if not 1 <= slots <= self.SLOT_MAX_ROWS:
+            raise ValueError("a slot cache holds 1..%d rows" % self.SLOT_MAX_ROWS)
+        capacity = int(capacity)
+        if not 1 <= capacity <= self.max_positions():
+            raise ValueError("capacity %d outside 1..%d" % (capacity, self.max_positions()))
+        if dtype == torch.bfloat16:
+            raise ValueError("this decoder's keys and values are fp16")
+        pages = slots * -(-capacity // page) if pages is None else int(pages)
+        dev = device if device is not None else self.embed_tokens.weight.device
+        cfg = self.cfg
+        return PagedSlots(cfg.decoder_layers, slots, capacity, cfg.decoder_attention_heads, cfg.head_dim, pages,
+                          page, dtype, window, sinks, dev)
+
+    def extend(self, cache: PagedSlots, entries, want=None, want_all=False):
+        """Runs the next tokens of several slots of a paged cache in one pass: ``entries`` is a list of (slot, ids), ids
+        a 1-D device tensor (or a list) without pads that continues what the slot holds - prompts, portions of them and
+        single tokens in any mix.  ``want``: per entry the offsets among its tokens whose logits are returned, fp16
+        [sum of wanted, vocab] in that order (None: no logits; ``want_all``: every token's).  More than PORTION tokens
+        run in portions."""
+        segments, ids = [], []
+        cache.exact_lens([slot for slot, _ in entries])
+        for slot, t in entries:
+            if not 0 <= slot < cache.batch:
+                raise ValueError("slot %d outside 0..%d" % (slot, cache.batch - 1))
+            t = t if torch.is_tensor(t) else upload(list(t), torch.long, cache.device)
+            if t.dim() != 1 or t.numel() == 0 or not t.is_cuda:
+                raise AssertionError("tokens must be non-empty 1-D device tensors")
+            segments.append((slot, max(0, cache.host_lens[slot]), t.numel()))
+            ids.append(t.long())
+        if len({s for s, _, _ in segments}) != len(segments):
+            raise ValueError("a slot is named twice")
+        if want_all:
+            want = [range(n) for _, _, n in segments]
+        if want is not None and any(not 0 <= k < n for (_, _, n), w in zip(segments, want) for k in w):
+            raise ValueError("a wanted place lies outside the entry's tokens")
+        cache.reserve(segments)
+        V, outs, order = self.cfg.vocab_size, [], []
+        # passes of at most PORTION tokens: whole entries, then pieces of the one that does not fit
+        passes, room = [[]], self.PORTION
+        for e, (slot, pos, n) in enumerate(segments):
+            at = 0
+            while at < n:
+                if room == 0:
+                    passes.append([])
+                    room = self.PORTION
+                m = min(room, n - at)
+                passes[-1].append((e, at, m))
+                at, room = at + m, room - m
+        for rows in passes:
+            if not rows:
+                continue
+            got = self._extend_pass(cache, [(segments[e][0], segments[e][1] + at, m) for e, at, m in rows],
+                                    torch.cat([ids[e][at:at + m] for e, at, m in rows]) if len(rows) > 1
+                                    else ids[rows[0][0]][rows[0][1]:rows[0][1] + rows[0][2]],
+                                    None if want is None else
+                                    [[k - at for k in want[e] if at <= k < at + m] for e, at, m in rows])
+            if got is not None:
+                outs.append(got)
+                order += [(e, k) for e, at, m in rows for k in want[e] if at <= k < at + m]
+        if want is None:
+            return None
+        if not outs:
+            return torch.empty(0, V, dtype=torch.float16, device=cache.device)
+        logits = outs[0] if len(outs) == 1 else torch.cat(outs)
+        wanted = [(e, k) for e, w in enumerate(want) for k in w]
+        if wanted != order:   # (an entry in several passes, its places in another order than its tokens)
+            place = {}
+            for i, ek in enumerate(order):
+                place.setdefault(ek, i)
+            logits = logits[upload([place[ek] for ek in wanted], torch.long, cache.device)]
+        return logits
+
+    def _extend_pass(self, cache, segments, flat, want):
+        lib = self.prepare_()
+        counts = [n for _, _, n in segments]
+        slots, starts = [s for s, _, _ in segments], [p for _, p, _ in segments]
+        M = sum(counts)
+        positions = np.concatenate([np.arange(p, p + n, dtype=np.int32) for _, p, n in segments])
+        pos = torch.from_numpy(positions).pin_memory().to(cache.device, non_blocking=True)
+        whole = slots == list(range(cache.batch))
+        table = cache.table if whole else cache.table.index_select(0, upload(slots, torch.long, cache.device))
+        layer = cache.layers[0]
+        batch = layer.batch(counts, starts, table)
+        paged = PagedRows(lib, cache, batch, self.cfg.decoder_attention_heads, self.cfg.head_dim, cache.device)
+        few = M <= 64 and want is not None and all(list(w) == list(range(n)) for w, n in zip(want, counts))
+        h, _ = self._rows_core(lib, _capi.stream_ptr(), flat.contiguous().view(M, 1), M, 1, 1, 0, None, None,
+                               len_dev=pos, paged=paged, want_packed=few)
+        for slot, p, n in segments:
+            cache.holds(slot, p + n)
+        cache.lens[upload(slots, torch.long, cache.device)] = upload([p + n for _, p, n in segments], torch.int32,
+                                                                    cache.device)
+        if want is None:
+            return None
+        if few:
+            return self._project(h, True, 1, M)[0]
+        first = np.concatenate([[0], np.cumsum(counts)])
+        rows = [int(first[e]) + k for e, w in enumerate(want) for k in w]
+        if not rows:
+            return None
+        if rows != list(range(M)):
+            h = h.index_select(0, upload(rows, torch.long, cache.device))
+        return self._project(h, False, 1, len(rows))[0]
+
+    def _decode_paged(self, cache, tokens, stream, lib):
+        """One token for every slot of a paged cache (pads and empty slots sit the step out)."""
+        B = cache.batch
+        # (a slot that pads have kept below what the host counts already has its next position's page)
+        active = [(s, n) for s, n in enumerate(cache.host_lens) if 0 <= n < cache.capacity]
+        cache.reserve([(s, n, 1) for s, n in active])
+        fixed = cache.__dict__.get("_decode_rows")
+        step_len = cache.__dict__.setdefault("step_len", torch.empty(B, dtype=torch.int32, device=cache.device))
+        bound = max((n + 1 for _, n in active), default=1)
+        if fixed is None or fixed[0] < bound or fixed[0] > 2 * bound + 512:
+            bound = min(cache.capacity, bound + 256)    # (how keys are split follows from it)
+            batch = cache.layers[0].batch([1] * B, step_len, cache.table, key_bound=bound)
+            fixed = cache._decode_rows = (bound, PagedRows(lib, cache, batch, self.cfg.decoder_attention_heads,
+                                                           self.cfg.head_dim, cache.device))
+        feat, _ = self._rows_core(lib, stream, tokens, B, 1, 1, 0, None, None, len_dev=cache.lens, step_len=step_len,
+                                  paged=fixed[1], want_packed=B <= 64)
+        check(lib.msa_advance_len(ptr(cache.lens), ptr(step_len), B, 1, stream))
+        for s, n in active:
+            cache.host_lens[s] = n + 1
+            cache.stale.add(s)
+        return feat
+
     def prefill_slot(self, cache: KVCache, slot: int, tokens: torch.Tensor):
         """Runs the prompt ``tokens`` (1-D ids on the device, no pads, the leading
         end-of-sentence token included) through the model into row ``slot`` of ``cache`` and
@@ -1006,6 +1153,9 @@ class TransformerDecoder(IncrementalDecoder):
                              % (T, cache.capacity))
         if not (cache.ragged and 0 <= slot < cache.batch):
             raise ValueError("not a slot cache, or slot %d outside 0..%d" % (slot, cache.batch - 1))
+        if isinstance(cache, PagedSlots):
+            self.release_slot(cache, slot)
+            return self.extend(cache, [(slot, tokens)], want_all=True)
         toks = tokens.long().contiguous().view(1, T)
         h, _ = self._rows_core(lib, _capi.stream_ptr(), toks, 1, T, T, 0, _SlotView(cache, slot),
                                None, want_packed=T <= 64)
@@ -1039,6 +1189,10 @@ class TransformerDecoder(IncrementalDecoder):
                                  % (slot, cache.batch - 1))
         if len(set(slots)) != len(slots):
             raise ValueError("a slot is named twice")
+        if isinstance(cache, PagedSlots):
+            for slot in slots:
+                self.release_slot(cache, slot)
+            return list(self.extend(cache, list(zip(slots, prompts)), want_all=True).split(lens))
         k, Tmax = len(prompts), max(lens)
         dev = prompts[0].device
         toks = torch.full((k, Tmax), self.padding_idx, dtype=torch.long, device=dev)
@@ -1079,7 +1233,11 @@ class TransformerDecoder(IncrementalDecoder):
             raise AssertionError("last_tokens must be int64 [%d]" % B)
         if sampled is not None and logits_out is None:
             raise AssertionError("sampled rows need logits_out")
-        if B > self.PACKED_MAX_ROWS:
+        if isinstance(cache, PagedSlots):
+            feat = self._decode_paged(cache, last_tokens.view(B, 1), stream, lib)
+            self._select_from(lib, feat, B, temperature, banned, stop, finished, row_mode, False, eos, tok_out, 1,
+                              score_out, 1, logits_out, packed=B <= 64)
+        elif B > self.PACKED_MAX_ROWS:
             # row-major activations through the tile kernels (int8 weights: chunks of <= 128
             # rows through the packed path), stored logits, stand-alone selection
             tokens = last_tokens.view(B, 1)

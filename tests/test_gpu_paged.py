@@ -500,3 +500,31 @@ def test_packed_outputs(rows):
     assert rc == 0, cache._lib.msa_last_error()
     got = out.view(8, mb, 4, 16, 8).permute(1, 3, 0, 2, 4).reshape(mb * 16, 256)
     assert torch.equal(got[:rows], want)
+
+
+def test_batches_without_rows():
+    cache = _cache(_pages(torch.float16, 2, 2, 16, 64, 70))
+    before = _host(cache)
+    for seqs in (0, 3):
+        b = cache.batch([0] * seqs, [0] * seqs, torch.zeros(seqs, 1, dtype=torch.int32, device=DEV))
+        e = torch.empty(0, 2, 64, dtype=torch.float16, device=DEV)
+        cache.append(b, e, e)
+        assert cache.attend(b, e).shape == (0, 2, 64) and cache.read(b)[0].shape == (0, 2, 64)
+    assert torch.equal(_host(cache)[0], before[0]) and torch.equal(_host(cache)[1], before[1])
+
+
+@pytest.mark.parametrize("new", [1, 60])
+def test_windows_of_any_size(new):
+    """From those that hold nothing but the row's own position to the largest number."""
+    cache = _cache(_pages(torch.bfloat16, 40, 1, 16, 64, 71))
+    table = _table(1, [40], 40, 72).to(DEV)
+    b = cache.batch([new], [570], table)
+    q = torch.randn(new, 2, 64, generator=torch.Generator().manual_seed(73)).bfloat16().to(DEV)
+    want = cache.attend(b, q)
+    for window in (570 + new, 640, 641, 2 ** 30, 2 ** 31 - 1):
+        for sinks in (0, 2 ** 31 - 1):
+            assert torch.equal(cache.attend(b, q, window=window, sinks=sinks), want), window
+    own = cache.attend(b, q, window=1)
+    v = cache.read(b)[1].expand(new, 2, 64) if new == 1 else cache.read(b)[1].expand(-1, 2, -1)
+    assert torch.equal(own, v)
+    assert torch.equal(cache.attend(b, q, window=1, sinks=2 ** 31 - 1), want)

@@ -62,7 +62,7 @@ BAD_CACHES = [dict(dtype=_capi.MSA_F32), dict(dtype=7), dict(format=3), dict(for
               dict(v_pages=None), dict(k_pages=4100), dict(format=1), dict(format=2, k_exp=ONE),
               dict(format=2, k_exp=ONE, v_exp=4097)]
 BAD_BATCHES = [dict(M=-1), dict(nseq=-1), dict(max_count=-1), dict(key_bound=-1), dict(min_count=-1), dict(min_count=2), dict(blocks=0), dict(table_stride=15),
-               dict(blocks=1 << 26, table_stride=1 << 26), dict(nseq=(1 << 20) + 1), dict(seq_start=None), dict(seq_pos=None),
+               dict(blocks=(1 << 24) + 1, table_stride=1 << 25), dict(nseq=(1 << 20) + 1), dict(seq_start=None), dict(seq_pos=None),
                dict(table=None)]
 BAD_ARGS = [dict(heads=0), dict(heads=6), dict(heads=-4), dict(q=None), dict(out=None), dict(q=4100), dict(out=4104),
             dict(ldq=1016), dict(ldq=1028), dict(ldo=1000), dict(ldo=1025), dict(window=-1), dict(sinks=-1), dict(scale=0.0),
@@ -99,7 +99,7 @@ def test_bad_rows_are_refused(k, ldk, v, ldv):
 def test_nothing_to_do_needs_no_gpu():
     lib = _capi.load()
     for b in (_batch(M=0), _batch(nseq=0), _batch(max_count=0, min_count=0)):
-        assert lib.msa_paged_append(ctypes.byref(_cache()), ctypes.byref(b), ONE, 512, ONE, 512, None) == 0
+        assert lib.msa_paged_append(ctypes.byref(_cache()), ctypes.byref(b), None, 512, None, 512, None) == 0
         assert lib.msa_paged_read(ctypes.byref(_cache()), ctypes.byref(b), ONE, 512, ONE, 512, None) == 0
         assert lib.msa_paged_attention(ctypes.byref(_cache()), ctypes.byref(b), ctypes.byref(_args()), None) == 0
         assert lib.msa_paged_attention_workspace_bytes(ctypes.byref(_cache()), ctypes.byref(b), ctypes.byref(_args())) == 0
