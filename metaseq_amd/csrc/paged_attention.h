@@ -515,7 +515,7 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
   }
 }
 
-// ---- portions of prompts: more than PA_FEW rows (token, query head) of a key/value head in a sequence ----------------
+// ---- portions of prompts: more than `few` rows (token, query head) of a key/value head in a sequence ----------------
 // Workgroup = 128 rows, 4 waves of 32; tiles of 64 keys go through LDS, two of keys and two of values, one barrier a
 // tile.  Everything transposed as above, with v_mfma 32x32x16: a lane has row n = lane % 32 and, with hl = lane / 32, 16 of 32
 // keys.  Row m of a block of S^T stands for the key with bits 2 and 3 of m exchanged, so that the eight probabilities
@@ -524,7 +524,6 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
 // ones through registers, where they become fp16: keys times 2^(e - the tile's largest e), values times 2^(e - E), E the largest so
 // far.  Chunks of 16 bytes of a row are exchanged by the row's number, so that reads of many rows meet all banks.
 constexpr int PT_BM = 128, PT_BN = 64, PT_THREADS = 256;
-constexpr int PA_FEW = 32;  // rows that the wave kernel above takes
 
 typedef __attribute__((address_space(3))) void pt_lds_void;
 
@@ -693,59 +692,52 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
   // whether any row of the workgroup sees the key
   const int g_lo = position(rho0), g_hi = position(rho0 + PT_BM - 1);
   auto anyone = [&](int key) { return pa_seen<1>(key, g_lo, g_hi, a.window, a.sinks) != 0; };
-  // 8 bits: chunks of 16 elements, registers in between
+  // 8 bits: chunks of 16 elements, registers in between.  Lane i of every wave has the exponents of key i; the factors that
+  // follow from them reach the lanes that need them through LDS of the wave's own.
   constexpr int CB = HD / 16, KN = (PT_BN * CB + PT_THREADS - 1) / PT_THREADS, VN = (HD * 4 + PT_THREADS - 1) / PT_THREADS;
-  pg_u4 kr[B8 ? KN : 1], vr[B8 ? VN : 1], vx;
-  int kx[B8 ? KN : 1], ke = 0, ve = 0;  // the rows' exponents; those of key `lane` of the tile
+  __shared__ __attribute__((aligned(16))) half_t s_factor[B8 ? PT_THREADS / 64 : 1][2][64];
+  pg_u4 kr[B8 ? KN : 1], vr[B8 ? VN : 1];
+  int ke = 0, ve = 0;
   const int vg = threadIdx.x & 3;       // the sixteen keys that the thread's chunks of V belong to
   auto fetch = [&](int i, PtPages pg) {
-    const int key0 = tiles.tile(i) * PT_BN;
+    const int key0 = tiles.tile(i) * PT_BN, in = page - 1;
 #pragma unroll
     for (int j = 0; j < KN; ++j) {
       const int at = min((int)threadIdx.x + j * PT_THREADS, PT_BN * CB - 1), row = at / CB, c = at % CB;
-      const int64_t up = ((int64_t)max(pg.of(row >> 4), 0) * a.kv_heads + h) * page + ((key0 + row) & (page - 1));
-      kr[j] = *(const pg_u4*)((const char*)a.k_pages + up * HD + c * 16);
-      kx[j] = a.k_exp[up];
+      kr[j] = *(const pg_u4*)((const char*)a.k_pages + h * unit + max(pg.of(row >> 4), 0) * page_bytes + ((key0 + row) & in) * HD + c * 16);
     }
-    const int64_t uv = (int64_t)max(pg.of(vg), 0) * a.kv_heads + h;
-    const int in = (key0 + vg * 16) & (page - 1);
+    const char* from = (const char*)a.v_pages + h * unit + max(pg.of(vg), 0) * page_bytes + ((key0 + vg * 16) & in);
 #pragma unroll
-    for (int j = 0; j < VN; ++j) {
-      const int row = min((int)threadIdx.x + j * PT_THREADS, HD * 4 - 1) >> 2;
-      vr[j] = *(const pg_u4*)((const char*)a.v_pages + uv * unit + (int64_t)row * page + in);
-    }
-    vx = *(const pg_u4*)(a.v_exp + uv * page + in);
-    const int64_t ul = ((int64_t)max(pg.of(lane >> 4), 0) * a.kv_heads + h) * page + ((key0 + lane) & (page - 1));
+    for (int j = 0; j < VN; ++j) vr[j] = *(const pg_u4*)(from + (min((int)threadIdx.x + j * PT_THREADS, HD * 4 - 1) >> 2) * page);
+    const int64_t ul = ((int64_t)max(pg.of(lane >> 4), 0) * a.kv_heads + h) * page + ((key0 + lane) & in);
     ke = a.k_exp[ul];
     ve = a.v_exp[ul];
   };
-  auto wave_most = [](int v) { return (int)wave_max((float)v); };
+  auto wave_most = [](int v) { return __builtin_amdgcn_readfirstlane((int)wave_max((float)v)); };
   // (returns the exponents that the tile's keys and values are relative to)
   auto stage = [&](int i, int slot, PtPages pg, int& ek, int& ev) {
     const int key0 = tiles.tile(i) * PT_BN;
     const bool mine = pg.of(lane >> 4) >= 0 && anyone(key0 + lane);
-    ek = __builtin_amdgcn_readfirstlane(wave_most(mine ? ke : -127));
-    ev = max(ev, __builtin_amdgcn_readfirstlane(wave_most(mine ? ve : -127)));
+    ek = wave_most(mine ? ke : -127);
+    ev = max(ev, wave_most(mine ? ve : -127));
+    // 2^(e - largest), 0 below what fp16 can be
+    auto factor = [](int e) { return e < -24 ? (half_t)0.f : (half_t)__builtin_bit_cast(float, (uint32_t)(127 + min(e, 0)) << 23); };
+    s_factor[wave][0][lane] = factor(ke - ek);
+    s_factor[wave][1][lane] = factor(ve - ev);
     char* kt = lds + slot * TILEB;
     char* vt = lds + (2 + slot) * TILEB;
-    auto power = [](int e) { return ldexpf(1.f, min(max(e, -126), 0)); };
 #pragma unroll
     for (int j = 0; j < KN; ++j) {
       const int at = threadIdx.x + j * PT_THREADS, row = at / CB, c = at % CB;
       if ((PT_BN * CB) % PT_THREADS == 0 || at < PT_BN * CB) {
-        const half_t f = (half_t)power(kx[j] - ek);
+        const half_t f = s_factor[wave][0][row & 63];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          half8_t w = __builtin_bit_cast(half8_t, pa_operand<F>(kr[j], e));
-          w *= f;
-          *(half8_t*)(kt + row * ROWB + pt_place<CH>(2 * c + e, row) * 16) = w;
-        }
+        for (int e = 0; e < 2; ++e)
+          *(half8_t*)(kt + row * ROWB + pt_place<CH>(2 * c + e, row) * 16) = __builtin_bit_cast(half8_t, pa_operand<F>(kr[j], e)) * f;
       }
     }
-    half8_t f[2];
+    const half8_t f[2] = {*(const half8_t*)&s_factor[wave][1][vg * 16], *(const half8_t*)&s_factor[wave][1][vg * 16 + 8]};
     const uint32_t seen = pg.of(vg) >= 0 ? pa_seen<16>(key0 + vg * 16, g_lo, g_hi, a.window, a.sinks) : 0;
-#pragma unroll
-    for (int k = 0; k < 16; ++k) f[k >> 3][k & 7] = (half_t)power((int)(int8_t)(vx[k >> 2] >> ((k & 3) * 8)) - ev);
 #pragma unroll
     for (int j = 0; j < VN; ++j) {
       const int at = threadIdx.x + j * PT_THREADS, row = at >> 2;

@@ -11,31 +11,40 @@ PAGED_FORMAT(i8)
 
 namespace {
 
-// out = sum of the splits' sums, each relative to its own maximum.  Workgroup = (token, query head); groups of hd / 4 threads
-// take every so manieth split, and their sums are added in the groups' order.  tokens: of the sequences of the wave kernel, at
-// most so many each; 0: every row of those of the tile kernel.
-constexpr int PC_THREADS = 256;
+// out = sum of the splits' sums, each relative to its own maximum.  hd / 4 threads have a (token, query head): a workgroup
+// takes several of them, or (MANY) one, for which groups of hd / 4 threads take every so manieth split and their sums are
+// added in the groups' order.  tokens: of the sequences of the wave kernel, at most so many each; 0: every row of those of
+// the tile kernel.
+constexpr int PC_THREADS = 256, PC_MANY = 9;
+template <bool MANY>
 __global__ __launch_bounds__(PC_THREADS) void paged_combine_kernel(PagedAttention a, int hd, int tokens) {
-  __shared__ __attribute__((aligned(16))) float s_o[PC_THREADS][4];
-  __shared__ float s_l[PC_THREADS];
-  const int lane = threadIdx.x & 63, head = blockIdx.y, splits = a.splits;
+  __shared__ __attribute__((aligned(16))) float s_o[MANY ? PC_THREADS : 1][4];
+  __shared__ float s_l[MANY ? PC_THREADS : 1];
+  const int lane = threadIdx.x & 63, splits = a.splits;
   const int s = tokens > 0 ? blockIdx.x / tokens : __builtin_amdgcn_readfirstlane(paged_sequence_of(a.seq_start, a.nseq, blockIdx.x));
   if (s >= a.nseq) return;
   const int row0 = a.seq_start[s], r = tokens > 0 ? row0 + (int)blockIdx.x - s * tokens : (int)blockIdx.x;
   const int count = min(min(a.seq_start[s + 1], a.M) - row0, a.max_count);
   if (a.seq_pos[s] < 0 || row0 < 0 || r - row0 >= count || (count * (a.heads / a.kv_heads) <= a.few) != (tokens > 0)) return;
   const int stride = hd + 4, columns = hd / 4, groups = PC_THREADS / columns;
+  const int g = threadIdx.x / columns, c = threadIdx.x - g * columns;
+  const int head = MANY ? blockIdx.y : blockIdx.y * groups + g;
+  if (!MANY && (g >= groups || head >= a.heads)) return;
   const float* part = a.partial + ((int64_t)r * a.heads + head) * splits * stride;
   float top = -INFINITY;
-  for (int i = lane; i < splits; i += 64) top = fmaxf(top, part[i * stride + hd]);
-  top = wave_max(top);
+  if constexpr (MANY) {
+    for (int i = lane; i < splits; i += 64) top = fmaxf(top, part[i * stride + hd]);
+    top = wave_max(top);
+  } else {
+#pragma unroll 4
+    for (int i = 0; i < splits; ++i) top = fmaxf(top, part[i * stride + hd]);
+  }
   const float off = top == -INFINITY ? 0.f : top;
-  const int g = threadIdx.x / columns, c = threadIdx.x - g * columns;
   float4_t o = {0.f, 0.f, 0.f, 0.f};
   float total = 0.f;
   if (g < groups) {
 #pragma unroll 4
-    for (int i = g; i < splits; i += groups) {
+    for (int i = MANY ? g : 0; i < splits; i += MANY ? groups : 1) {
       const float4_t v = *(const float4_t*)(part + i * stride + c * 4);
       const float w = __builtin_amdgcn_exp2f(part[i * stride + hd] - off);
       total += w * part[i * stride + hd + 1];
@@ -43,15 +52,17 @@ __global__ __launch_bounds__(PC_THREADS) void paged_combine_kernel(PagedAttentio
       for (int k = 0; k < 4; ++k) o[k] += w * v[k];
     }
   }
-  *(float4_t*)s_o[threadIdx.x] = o;
-  s_l[threadIdx.x] = total;
-  __syncthreads();
-  if ((int)threadIdx.x >= columns) return;
-  for (int i = 1; i < groups; ++i) {
-    const float4_t v = *(const float4_t*)s_o[i * columns + c];
-    total += s_l[i * columns + c];
+  if constexpr (MANY) {
+    *(float4_t*)s_o[threadIdx.x] = o;
+    s_l[threadIdx.x] = total;
+    __syncthreads();
+    if ((int)threadIdx.x >= columns) return;
+    for (int i = 1; i < groups; ++i) {
+      const float4_t v = *(const float4_t*)s_o[i * columns + c];
+      total += s_l[i * columns + c];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) o[k] += v[k];
+      for (int k = 0; k < 4; ++k) o[k] += v[k];
+    }
   }
   const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
   uint16_t w[4];
@@ -63,8 +74,14 @@ __global__ __launch_bounds__(PC_THREADS) void paged_combine_kernel(PagedAttentio
   *(pg_u2*)((uint16_t*)a.out + at) = pg_u2{(uint32_t)w[0] | (uint32_t)w[1] << 16, (uint32_t)w[2] | (uint32_t)w[3] << 16};
 }
 
-// How a batch is taken: sequences of at most PA_FEW rows (token, query head) of a key/value head by the wave kernel, others
-// by tiles; each splits keys over workgroups where there are few of those.
+// How a batch is taken: sequences of at most few_of() rows (token, query head) of a key/value head by the wave kernel, others
+// by tiles; each splits keys over workgroups where there are few of those.  The wave kernel reads the keys once per 32 rows;
+// a tile costs the same up to 128, and with 8 bits more, as its operands are made in registers and cross LDS (us, waves and
+// tiles, 128 dimensions, 32 query heads: fp16 of as many key/value heads, 16 sequences of 2000 keys, 32 rows 85 and 89, 48
+// 116 and 93; 64 sequences of 1000 keys 164 and 183, 211 and 193; 8 heads, 16 sequences 38 and 39, 37 and 40; e4m3, 64 rows
+// 98 and 138, 96 rows 138 and 139; 64 sequences 251 and 264, 346 and 281; 8 heads 70 and 75, 97 and 77).
+int few_of(const msa_paged_cache& c) { return c.format == MSA_PAGES_SAME ? 32 : 64; }
+
 struct Plan {
   int row_tiles, row_blocks, splits;  // wave kernel (row_tiles 0: not launched)
   int tile_blocks, tile_splits, grouped;  // tile kernel (tile_blocks 0: not launched)
@@ -81,6 +98,18 @@ int splits_of(int64_t groups, int64_t tiles, int64_t least) {
   return s < 1 ? 1 : (int)s;
 }
 
+// The same for tiles: up to one workgroup a CU, of at least 4 tiles each; twice as many, two a CU (where registers and LDS
+// allow that, dimensions of up to 128), if each still has more than 16.  (us in 1, 2, 4, 8, 16 splits: 16 workgroups over 4064
+// keys 108, 64, 41, 32, 28; 64 over 4064 110, 64, 41, 36, 48; 128 over 8704 227, 131, 102, 115, 150; 256 over 9216 256, 191, 198,
+// 231; 256 over 1024 37, 39, 47; of 256 dimensions 32 over 4064 217, 121, 72, 50, 60)
+int tile_splits_of(int64_t groups, int64_t tiles, int hd) {
+  int64_t s = 256 / groups;
+  if (s > tiles / 4) s = tiles / 4;
+  if (s < 1) s = 1;
+  if (hd <= 128 && groups * s <= 256 && tiles > 16 * s) s *= 2;
+  return s > 128 ? 128 : (int)s;
+}
+
 Plan plan_of(const msa_paged_cache& c, const msa_paged_batch& b, const msa_paged_attention_args& a) {
   Plan p = {0, 0, 1, 0, 1, 0};
   const int group = a.heads / c.kv_heads;
@@ -90,19 +119,25 @@ Plan plan_of(const msa_paged_cache& c, const msa_paged_batch& b, const msa_paged
     const int64_t span = (int64_t)a.window + a.sinks + tokens;
     return a.window > 0 && span < b.key_bound ? span : (int64_t)b.key_bound;
   };
-  if ((int64_t)b.min_count * group <= PA_FEW) {
-    const int64_t most = rows < PA_FEW ? rows : PA_FEW;
+  const int few = few_of(c);
+  if ((int64_t)b.min_count * group <= few) {
+    const int64_t most = rows < few ? rows : few;
     p.row_tiles = most <= 16 ? 1 : 2;
     p.row_blocks = (int)((most + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
     const int kt = c.format == MSA_PAGES_SAME ? 32 : 64;
     const int64_t units = (int64_t)b.nseq * p.row_blocks * c.kv_heads;
     p.splits = splits_of(units, (keys_of(most) + kt - 1) / kt, PA_NW);
   }
-  if (rows > PA_FEW) {
+  if (rows > few) {
     p.tile_blocks = (int)((rows + PT_BM - 1) / PT_BM);
     const int64_t units = (int64_t)b.nseq * c.kv_heads;
-    p.tile_splits = splits_of(units * p.tile_blocks, (keys_of(PT_BM / group + 1) + PT_BN - 1) / PT_BN, 8);
-    p.grouped = units % 8 == 0 || units >= 64;
+    p.tile_splits = tile_splits_of(units * p.tile_blocks, (keys_of(PT_BM / group + 1) + PT_BN - 1) / PT_BN, c.hd);
+    // A (sequence, head)'s blocks one after another on one XCD, whose L2 then has its keys, where all have about as many:
+    // with the long blocks of every unit first the short ones fill the end (us, units first and blocks first: 64 units of 16
+    // blocks behind 4096 keys 257 and 301, of 32 behind 1024 204 and 218; 16 units of 128 with a window 178 and 190; from the
+    // first key on 32 units of 32 blocks 223 and 178, 256 of 16 314 and 303).  Workgroups go to the XCDs in turn, so that
+    // multiples of 8 units keep theirs either way.
+    p.grouped = units % 8 == 0 && p.tile_blocks >= 8 && keys_of(b.max_count) >= 2 * (int64_t)(a.window > 0 ? 0 : b.max_count);
   }
   return p;
 }
@@ -156,20 +191,22 @@ extern "C" int msa_paged_attention(const msa_paged_cache* c, const msa_paged_bat
               "msa_paged_attention: the workspace has %lld bytes, %lld are needed", (long long)a->workspace_bytes, (long long)need);
   const Plan p = plan_of(*c, *b, *a);
   const int64_t units = (int64_t)b->nseq * c->kv_heads;
-  MSA_REQUIRE((int64_t)b->nseq * PA_FEW <= INT32_MAX && units * p.row_blocks <= INT32_MAX && (units + 7) * p.tile_blocks * p.tile_splits <= INT32_MAX,
+  MSA_REQUIRE((int64_t)b->nseq * few_of(*c) <= INT32_MAX && units * p.row_blocks <= INT32_MAX && (units + 7) * p.tile_blocks * p.tile_splits <= INT32_MAX,
               MSA_ERR_INVALID_ARG, "msa_paged_attention: too many rows for one call");
   // (positions are below 2^30; a window that holds them all is none)
   const int window = a->window < (int64_t)b->blocks * c->page ? a->window : 0;
   PagedAttention k = {a->q, c->k_pages, c->v_pages, c->k_exp, c->v_exp, b->seq_start, b->seq_pos, b->table, a->ldq, a->ldo,
                       b->table_stride, a->out, (float*)a->workspace, b->M, b->nseq, a->heads, c->kv_heads, c->pages,
                       paged_log2(c->page), b->blocks, a->out_mb, window, a->sinks, 1, 1,
-                      c->dtype == MSA_BF16, b->max_count, PA_FEW, p.grouped, a->scale};
+                      c->dtype == MSA_BF16, b->max_count, few_of(*c), p.grouped, a->scale};
   hipStream_t s = (hipStream_t)stream;
   const int format = paged_format(*c);
   auto combine = [&](int tokens) {
     if (k.splits == 1) return;
-    hipLaunchKernelGGL(paged_combine_kernel, dim3((unsigned)(tokens > 0 ? b->nseq * tokens : b->M), (unsigned)a->heads),
-                       dim3(PC_THREADS), 0, s, k, c->hd, tokens);
+    const unsigned x = (unsigned)(tokens > 0 ? b->nseq * tokens : b->M);
+    const int each = PC_THREADS / (c->hd / 4);
+    if (k.splits >= PC_MANY) hipLaunchKernelGGL(paged_combine_kernel<true>, dim3(x, (unsigned)a->heads), dim3(PC_THREADS), 0, s, k, c->hd, tokens);
+    else hipLaunchKernelGGL(paged_combine_kernel<false>, dim3(x, (unsigned)((a->heads + each - 1) / each)), dim3(PC_THREADS), 0, s, k, c->hd, tokens);
   };
   if (p.tile_blocks > 0) {
     k.splits = p.tile_splits;
@@ -191,7 +228,7 @@ extern "C" int msa_paged_attention(const msa_paged_cache* c, const msa_paged_bat
       case PG_E4M3: msa_launch_paged_rows_e4m3(k, c->hd, p.row_tiles, s); break;
       default: msa_launch_paged_rows_i8(k, c->hd, p.row_tiles, s); break;
     }
-    const int few = PA_FEW / (a->heads / c->kv_heads);
+    const int few = k.few / (a->heads / c->kv_heads);
     combine(few < 1 ? 1 : few < b->max_count ? few : b->max_count);
     MSA_CHECK_LAUNCH("msa_paged_attention (rows)");
   }

@@ -165,7 +165,11 @@ __global__ __launch_bounds__(256) void read_rows_kernel(PagedRows a) {
 // prompts.  Rows are read and written 16 bytes a lane; values cross over in LDS, and leave (or come) as 16 bytes of one
 // dimension's consecutive positions.  Bound by HBM.
 constexpr int PB = 64;  // positions of a block
-constexpr int BLOCK_TOKENS = 8;
+// From this many new tokens of the longest sequence on the blocks are ahead of a wave for every row, which writes (or reads)
+// its values two bytes at a time.  (us, rows and blocks, 64 sequences of 72 heads of 128: fp16 append of 2 15 and 16, of 3 24
+// and 18, read of 2 21 and 25, of 3 32 and 26; e4m3 read of 2 12 and 14, of 3 18 and 14, append of 4 26 and 32, of 6 37 and 34;
+// a block's 8 bits cross LDS, and 256 sequences of 8 heads append 6 in 19 and 25, 12 in 30 and 29)
+constexpr int block_tokens(bool append, int format) { return append && (format == PG_E4M3 || format == PG_I8) ? 6 : 3; }
 
 struct Block {
   int first, begin, end, row;  // positions that are new: begin .. end - 1; the row of position `first`
@@ -420,8 +424,7 @@ __global__ __launch_bounds__(256) void read_block_kernel(PagedRows a, int blocks
 
 template <int DT, int F, int HD>
 void launch_rows_hd(const PagedRows& a, bool append, hipStream_t s) {
-  // (BLOCK_TOKENS: see below)
-  if (a.b.max_count < BLOCK_TOKENS) {
+  if (a.b.max_count < block_tokens(append, F)) {
     const dim3 grid((unsigned)a.b.M, (unsigned)((a.c.kv_heads + 3) / 4));
     if (append) hipLaunchKernelGGL((append_rows_kernel<DT, F>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((read_rows_kernel<DT, F>), grid, dim3(256), 0, s, a);

@@ -253,6 +253,13 @@ ATTENTION = [
     (2, 1, 256, 64, [70, 150], [100, 3], 0, 0),
     (3, 3, 192, 16, [90], [50], 20, 0),
     (2, 2, 80, 32, [128, 257], [0, 64], 0, 0),
+    # rows on both sides of 32 and of 64, which different kernels take, in one batch
+    (4, 2, 64, 16, [16, 17, 32, 33, 3], [0, 50, 7, 100, 20], 0, 0),
+    (3, 1, 128, 32, [21, 22, 11, 10], [100, 0, 33, 200], 40, 5),
+    (5, 5, 96, 64, [64, 65, 32, 33], [5, 0, 90, 2], 0, 0),
+    (4, 4, 256, 128, [33, 48], [120, 300], 0, 0),
+    # many blocks of eight heads behind as many keys
+    (8, 8, 64, 64, [1030], [1100], 0, 0),
 ]
 
 
@@ -324,7 +331,7 @@ def test_what_is_not_finite_reaches_the_rows_that_see_it(dtype, new):
 
 
 @pytest.mark.parametrize("form", [torch.float16, E4M3, torch.int8], ids=["f16", "e4m3", "i8"])
-@pytest.mark.parametrize("new,pos,window", [(1, 9000, 0), (3, 5000, 0), (1, 9000, 2500), (300, 2000, 0)])
+@pytest.mark.parametrize("new,pos,window", [(1, 9000, 0), (3, 5000, 0), (1, 9000, 2500), (300, 2000, 0), (50, 4000, 0), (20, 3000, 1500)])
 def test_long_histories(form, new, pos, window):
     """Keys split over workgroups; values and keys of very different sizes, zeros among them."""
     host = _pages(form, 160, 1, 64, 128, 20)
@@ -342,7 +349,7 @@ def test_long_histories(form, new, pos, window):
     cache = _cache(host)
     q = torch.randn(new, 4, 128, generator=g).half()
     out = cache.attend(cache.batch([new], [pos], table.to(DEV)), q.to(DEV), window=window, sinks=4).cpu()
-    if new > 8:  # the oracle goes row by row
+    if new > 100:  # a few rows, one by one
         keys, there = O.positions(host[0], host[2], table[0], pos + new, False)
         values, _ = O.positions(host[1], host[3], table[0], pos + new, True)
         for i in (0, 1, 150, 299):
