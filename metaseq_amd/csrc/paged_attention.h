@@ -562,6 +562,7 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
   constexpr bool B8 = X::bits8;
   constexpr int ES = X::ES;
   constexpr int KSTEPS = HD / 16, DBLK = (HD + 31) / 32;
+  constexpr int AHEAD = 2, VAHEAD = 2;  // fragments requested ahead: pairs of K, of V
   constexpr int CH = HD / 8;                    // 16-byte chunks of a key row in LDS, which holds 16-bit elements
   constexpr int ROWB = HD * 2, TILEB = PT_BN * ROWB;
   constexpr float SHIFT = X::SHIFT;
@@ -826,15 +827,28 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
     // Two copies: tiles that every row of the wave sees whole, and others.
     auto attend = [&](auto edge) {
       constexpr bool EDGE = decltype(edge)::value;
+      // (the order below is kept: left alone, the compiler requests a fragment right before its product and waits for it)
       float16_t sc[2];
+      pg_u4 kf[AHEAD][2], vf[VAHEAD];
+      auto k_at = [&](int ks, int ib) {
+        const int row = ib * 32 + krow;
+        return *(const pg_u4*)(kt + row * ROWB + pt_place<CH>(2 * ks + hl, row) * 16);
+      };
 #pragma unroll
-      for (int ks = 0; ks < KSTEPS; ++ks)
+      for (int ks = 0; ks < AHEAD; ++ks) kf[ks][0] = k_at(ks, 0), kf[ks][1] = k_at(ks, 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int ks = 0; ks < KSTEPS; ++ks) {
 #pragma unroll
         for (int ib = 0; ib < 2; ++ib) {
-          const int row = ib * 32 + krow;
-          const pg_u4 k = *(const pg_u4*)(kt + row * ROWB + pt_place<CH>(2 * ks + hl, row) * 16);
-          sc[ib] = pt_mfma<F>(k, qf[ks], ks == 0 ? zero16 : sc[ib]);
+          sc[ib] = pt_mfma<F>(kf[ks % AHEAD][ib], qf[ks], ks == 0 ? zero16 : sc[ib]);
+          if (ks + AHEAD < KSTEPS) kf[ks % AHEAD][ib] = k_at(ks + AHEAD, ib);
         }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int n = 0; n < VAHEAD; ++n) vf[n] = v_at(vt, n % DBLK, n / DBLK);
+      __builtin_amdgcn_sched_barrier(0);
       float z[32];  // keys key0 + 16 (j / 8) + 8 hl + j % 8
 #pragma unroll
       for (int j = 0; j < 32; ++j) z[j] = sc[j >> 4][j & 15];
@@ -871,25 +885,19 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
       const float off = (m == -INFINITY ? 0.f : m) - SHIFT;
       pg_u4 p[4];  // steps of sixteen keys of the product with V
       float sum[2] = {0.f, 0.f};  // of the probabilities as they are rounded
-#pragma unroll
-      for (int st = 0; st < 4; ++st) {
-        float e[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[st * 8 + j], c, -off));
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (F == PG_BF16) {
-            const bf16x2_t w = {(bf16_t)e[2 * j], (bf16_t)e[2 * j + 1]}, one = {(bf16_t)1.f, (bf16_t)1.f};
-            sum[j & 1] = __builtin_amdgcn_fdot2_f32_bf16(w, one, sum[j & 1], false);
-            p[st][j] = __builtin_bit_cast(uint32_t, w);
-          } else {
-            const half2_t w = {(half_t)e[2 * j], (half_t)e[2 * j + 1]}, one = {(half_t)1.f, (half_t)1.f};
-            sum[j & 1] = __builtin_amdgcn_fdot2(w, one, sum[j & 1], false);
-            p[st][j] = __builtin_bit_cast(uint32_t, w);
-          }
+      auto pair = [&](int st, int j) {
+        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(z[st * 8 + 2 * j], c, -off));
+        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(z[st * 8 + 2 * j + 1], c, -off));
+        if (F == PG_BF16) {
+          const bf16x2_t w = {(bf16_t)e0, (bf16_t)e1}, one = {(bf16_t)1.f, (bf16_t)1.f};
+          sum[j & 1] = __builtin_amdgcn_fdot2_f32_bf16(w, one, sum[j & 1], false);
+          p[st][j] = __builtin_bit_cast(uint32_t, w);
+        } else {
+          const half2_t w = {(half_t)e0, (half_t)e1}, one = {(half_t)1.f, (half_t)1.f};
+          sum[j & 1] = __builtin_amdgcn_fdot2(w, one, sum[j & 1], false);
+          p[st][j] = __builtin_bit_cast(uint32_t, w);
         }
-      }
-      l += sum[0] + sum[1];
+      };
       if (EDGE && F != PG_I8) {
         if (odd) {  // (an infinity or a NaN times a probability is itself)
 #pragma unroll 1
@@ -910,10 +918,14 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
         }
       }
 #pragma unroll
-      for (int st = 0; st < 4; ++st)
+      for (int j = 0; j < 4; ++j) pair(0, j);
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int db = 0; db < DBLK; ++db) {
-          pg_u4 v = v_at(vt, db, st);
+          const int n = st * DBLK + db;
+          pg_u4 v = vf[n % VAHEAD];
           if (EDGE && F != PG_I8) {
             if (odd) {
 #pragma unroll
@@ -921,7 +933,16 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
             }
           }
           o[db] = pt_mfma<F>(v, p[st], o[db]);
+          if (n + VAHEAD < 4 * DBLK) vf[n % VAHEAD] = v_at(vt, (n + VAHEAD) % DBLK, (n + VAHEAD) / DBLK);
+          if (st < 3) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (db == (DBLK > 4 ? j : j * DBLK / 4)) pair(st + 1, j);
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
+      }
+      l += sum[0] + sum[1];
     };
     if (whole) attend(std::false_type{});
     else if (!none) attend(std::true_type{});
