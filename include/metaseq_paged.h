@@ -37,9 +37,10 @@ typedef struct {
  * stay as they were); seq_pos [nseq]: position of its first row (negative: the sequence sits this call out, its
  * outputs stay as they were).  Position p of sequence s is in page table[s * table_stride + p / page]; positions
  * whose entry is outside 0 .. pages - 1, or beyond the `blocks` entries of a sequence, are nowhere: they are not written,
- * read back as zeros and seen by no row.  A table names at most 2^30 positions.  max_count: no sequence has more rows (those that it has beyond are left
- * alone); min_count: no sequence that has rows has fewer (0: not known); key_bound: no row's position reaches it (a hint: how keys are split follows from it, results up to
- * rounding do not). */
+ * read back as zeros and seen by no row.  A table names at
+ * most 2^30 positions, a batch has fewer than 2^24 rows.  max_count: no sequence has more rows (those that it has beyond
+ * are left alone); min_count: no sequence that has rows has fewer (0: not known); key_bound: no row's position reaches it
+ * (a hint: how keys are split follows from it, results up to rounding do not). */
 typedef struct {
   int M, nseq, max_count, min_count, key_bound, blocks;
   int64_t table_stride;
@@ -50,7 +51,8 @@ typedef struct {
  * = 448 (e4m3) or 127 (int8), e = the least integer >= -126 with max |x| <= top 2^e over the position's and
  * head's elements, c = x 2^-e rounded to nearest even.  Magnitudes beyond what c 2^e can stand for in dtype (1.875
  * times its largest power of two in e4m3, 1.984375 times it in int8), infinities too, are held as that; NaN is
- * held as e4m3's NaN, in int8 as 0, and is left out of the maximum.  Positions that two rows name get either's. */
+ * held as e4m3's NaN, in int8 as 0, and is left out of the maximum.  What a position holds that two rows of a call name is
+ * undefined (parts of both). */
 int msa_paged_append(const msa_paged_cache* c, const msa_paged_batch* b, const void* k, int64_t ldk, const void* v,
                      int64_t ldv, void* stream);
 
@@ -62,7 +64,8 @@ int msa_paged_read(const msa_paged_cache* c, const msa_paged_batch* b, void* k, 
  * head h uses key/value head h / (heads / kv_heads).  The row at position i sees positions j <= i, with window > 0 only
  * those of them with j > i - window or j < sinks:
  *   out = sum_j softmax_j(scale q . k_j) v_j
- * in fp32, rounded once; a row that sees nothing is zeros.  What stands at positions that no row of a sequence sees is never
+ * in fp32, rounded once; a row that sees nothing is zeros.  A row behind its table's positions sees what one at the last of
+ * them would.  What stands at positions that no row of a sequence sees is never
  * used, whatever it is.  q [M, heads, hd] with row stride ldq; out with row stride ldo, or (out_mb > 0, MSA_F16, M <=
  * 128) in the packed activation layout of metaseq_amd.h with that many row blocks of heads * hd columns.
  * workspace: at least msa_paged_attention_workspace_bytes of the same arguments (0: none needed), 16-byte aligned; calls

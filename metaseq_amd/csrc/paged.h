@@ -14,6 +14,11 @@ inline int paged_log2(int page) { return __builtin_ctz((unsigned)page); }
 
 int msa_paged_check(const msa_paged_cache* c, const msa_paged_batch* b, const char* who);
 
+// Tables name positions below 2^30: one from there on, whichever it is, is nowhere (and a batch's rows behind it are too).
+constexpr int PG_NOWHERE = 1 << 30;
+// Workgroups of 256 threads that one launch may have (2^32 threads), and rows of a batch.
+constexpr int PG_MOST_GROUPS = (1 << 24) - 1;
+
 // attention of a batch, one format of pages (paged_attention_*.hip)
 struct PagedAttention {
   const void* q;

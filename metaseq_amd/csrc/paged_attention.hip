@@ -191,7 +191,8 @@ extern "C" int msa_paged_attention(const msa_paged_cache* c, const msa_paged_bat
               "msa_paged_attention: the workspace has %lld bytes, %lld are needed", (long long)a->workspace_bytes, (long long)need);
   const Plan p = plan_of(*c, *b, *a);
   const int64_t units = (int64_t)b->nseq * c->kv_heads;
-  MSA_REQUIRE((int64_t)b->nseq * few_of(*c) <= INT32_MAX && units * p.row_blocks <= INT32_MAX && (units + 7) * p.tile_blocks * p.tile_splits <= INT32_MAX,
+  MSA_REQUIRE((int64_t)b->nseq * few_of(*c) <= PG_MOST_GROUPS && units * p.row_blocks <= PG_MOST_GROUPS &&
+                  (units + 7) * p.tile_blocks * p.tile_splits <= PG_MOST_GROUPS,
               MSA_ERR_INVALID_ARG, "msa_paged_attention: too many rows for one call");
   // (positions are below 2^30; a window that holds them all is none)
   const int window = a->window < (int64_t)b->blocks * c->page ? a->window : 0;

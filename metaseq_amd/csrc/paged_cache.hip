@@ -72,8 +72,8 @@ __global__ __launch_bounds__(256) void append_rows_kernel(PagedRows a) {
   if (h >= a.c.kv_heads) return;
   const int s = __builtin_amdgcn_readfirstlane(paged_sequence_of(a.b.seq_start, a.b.nseq, r));
   if (s >= a.b.nseq || r >= a.b.seq_start[a.b.nseq] || a.b.seq_pos[s] < 0 || r - a.b.seq_start[s] >= a.b.max_count) return;
-  const int p = a.b.seq_pos[s] + r - a.b.seq_start[s];
-  const int pg = p < 0 ? -1 : page_of(a, s, p);
+  const int p = min(a.b.seq_pos[s], PG_NOWHERE) + r - a.b.seq_start[s];
+  const int pg = page_of(a, s, p);
   if (pg < 0) return;
   const int hd = a.c.hd, page = 1 << a.page_log2, at = p & (page - 1);
   const int64_t unit = (int64_t)pg * a.c.kv_heads + h;  // of the page and head
@@ -138,8 +138,8 @@ __global__ __launch_bounds__(256) void read_rows_kernel(PagedRows a) {
   if (h >= a.c.kv_heads) return;
   const int s = __builtin_amdgcn_readfirstlane(paged_sequence_of(a.b.seq_start, a.b.nseq, r));
   if (s >= a.b.nseq || r >= a.b.seq_start[a.b.nseq] || a.b.seq_pos[s] < 0 || r - a.b.seq_start[s] >= a.b.max_count) return;
-  const int p = a.b.seq_pos[s] + r - a.b.seq_start[s];
-  const int pg = p < 0 ? -1 : page_of(a, s, p);
+  const int p = min(a.b.seq_pos[s], PG_NOWHERE) + r - a.b.seq_start[s];
+  const int pg = page_of(a, s, p);
   const int hd = a.c.hd, page = 1 << a.page_log2, at = p & (page - 1);
   T* k = (T*)a.k_out + (int64_t)r * a.ldk + h * hd;
   T* v = (T*)a.v_out + (int64_t)r * a.ldv + h * hd;
@@ -176,10 +176,10 @@ struct Block {
 };
 __device__ __forceinline__ bool block_of(const PagedRows& a, int s, int i, Block& b) {
   const pg_uniform_i32* start = (const pg_uniform_i32*)(uintptr_t)a.b.seq_start;
-  const int row0 = start[s], pos = ((const pg_uniform_i32*)(uintptr_t)a.b.seq_pos)[s];
+  const int row0 = start[s], pos = min(((const pg_uniform_i32*)(uintptr_t)a.b.seq_pos)[s], PG_NOWHERE);
   const int64_t count = min(min(start[s + 1], a.b.M) - row0, a.b.max_count);
   const int64_t first = ((int64_t)(pos >> 6) + i) * PB;
-  if (pos < 0 || row0 < 0 || count <= 0 || first >= pos + count || pos + count > INT32_MAX) return false;
+  if (pos < 0 || row0 < 0 || count <= 0 || first >= pos + count) return false;
   b.first = (int)first;
   b.begin = max(pos, b.first);
   b.end = (int)min(pos + count, first + PB);
@@ -468,7 +468,7 @@ int check_rows(const msa_paged_cache* c, const msa_paged_batch* b, const void* k
   MSA_REQUIRE(k && v, MSA_ERR_INVALID_ARG, "%s: null pointer", who);
   MSA_REQUIRE(((uintptr_t)k | (uintptr_t)v) % 16 == 0, MSA_ERR_INVALID_ARG, "%s: keys and values must be 16-byte aligned", who);
   const int64_t n = (int64_t)c->kv_heads * c->hd;
-  MSA_REQUIRE((int64_t)b->nseq * (((int64_t)b->max_count + 62) / 64 + 1) * c->kv_heads <= INT32_MAX, MSA_ERR_INVALID_ARG, "%s: too many rows for one call", who);
+  MSA_REQUIRE((int64_t)b->nseq * (((int64_t)b->max_count + 62) / 64 + 1) * c->kv_heads <= PG_MOST_GROUPS, MSA_ERR_INVALID_ARG, "%s: too many rows for one call", who);
   MSA_REQUIRE(ldk >= n && ldv >= n && ldk % 8 == 0 && ldv % 8 == 0, MSA_ERR_INVALID_ARG,
               "%s: row strides must be multiples of 8 of at least kv_heads * hd", who);
   return MSA_OK;
@@ -490,6 +490,7 @@ int msa_paged_check(const msa_paged_cache* c, const msa_paged_batch* b, const ch
   MSA_REQUIRE(c->format == MSA_PAGES_SAME || (c->k_exp && c->v_exp), MSA_ERR_INVALID_ARG, "%s: 8-bit pages need exponents", who);
   MSA_REQUIRE(((uintptr_t)c->k_pages | (uintptr_t)c->v_pages | (uintptr_t)c->k_exp | (uintptr_t)c->v_exp) % 16 == 0,
               MSA_ERR_INVALID_ARG, "%s: pages and exponents must be 16-byte aligned", who);
+  MSA_REQUIRE(b->M <= PG_MOST_GROUPS && b->max_count <= PG_MOST_GROUPS, MSA_ERR_INVALID_ARG, "%s: too many rows for one call", who);
   MSA_REQUIRE(b->M >= 0 && b->nseq >= 0 && b->nseq <= (1 << 20) && b->max_count >= 0 && b->key_bound >= 0, MSA_ERR_INVALID_ARG,
               "%s: negative sizes, or more than 2^20 sequences", who);
   MSA_REQUIRE(b->min_count >= 0 && b->min_count <= b->max_count, MSA_ERR_INVALID_ARG, "%s: min_count must be 0 .. max_count", who);

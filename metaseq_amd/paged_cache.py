@@ -132,7 +132,9 @@ class PagedCache:
         return PagedBatch(c, start[-1], seq_start, seq_pos, table)
 
     # ------------------------------------------------------------------ calls
-    def _of(self, dtype):
+    def _of(self, dtype, batch=None):
+        if batch is not None and batch.table.device != self.device:
+            raise ValueError("the batch is on %s, the pages are on %s" % (batch.table.device, self.device))
         if dtype not in self._c:
             raise ValueError("pages of %s hold no %s" % (self.k_pages.dtype, dtype))
         return self._c[dtype][1]
@@ -168,10 +170,10 @@ class PagedCache:
 
     def append(self, batch, k, v):
         """Stores the keys and values ([rows, kv_heads, head_dim], fp16 or bf16, any row stride) of a batch's tokens at
-        their positions."""
+        their positions.  Nothing of this class records gradients."""
         if k.dtype != v.dtype:
             raise ValueError("keys are %s, values %s" % (k.dtype, v.dtype))
-        c = self._of(k.dtype)
+        c = self._of(k.dtype, batch)
         k = self._rows("k", k, batch.rows, self.kv_heads, True)
         v = self._rows("v", v, batch.rows, self.kv_heads, True)
         self._run(self._lib.msa_paged_append, c, batch.by_ref, k.data_ptr(), self._ld(k), v.data_ptr(), self._ld(v))
@@ -186,7 +188,7 @@ class PagedCache:
             out = tuple(torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
         elif out[0].dtype != out[1].dtype or dtype not in (None, out[0].dtype):
             raise ValueError("keys and values come in one dtype")
-        c = self._of(out[0].dtype)
+        c = self._of(out[0].dtype, batch)
         k, v = (self._rows("out", t, batch.rows, self.kv_heads, False) for t in out)
         self._run(self._lib.msa_paged_read, c, batch.by_ref, k.data_ptr(), self._ld(k), v.data_ptr(), self._ld(v))
         return out
@@ -198,7 +200,9 @@ class PagedCache:
         holds (or are undefined)."""
         if q.dim() != 3 or q.shape[1] % self.kv_heads or q.shape[1] == 0:
             raise ValueError("q must be [rows, heads, head_dim], heads a multiple of %d" % self.kv_heads)
-        c = self._of(q.dtype)
+        if not (0 <= window < 2 ** 31 and 0 <= sinks < 2 ** 31):
+            raise ValueError("window and sinks must be 0 .. 2^31 - 1")
+        c = self._of(q.dtype, batch)
         heads = q.shape[1]
         q = self._rows("q", q, batch.rows, heads, True)
         if out is None:
@@ -243,8 +247,8 @@ class PagedSlots:
         blocks = -(-capacity // page)
         self.batch, self.capacity, self.page, self.device = int(slots), int(capacity), int(page), device
         self.window, self.sinks = int(window), int(sinks)
-        if self.window < 0 or self.sinks < 0:
-            raise ValueError("window and sinks must not be negative")
+        if not (0 <= self.window < 2 ** 31 and 0 <= self.sinks < 2 ** 31):
+            raise ValueError("window and sinks must be 0 .. 2^31 - 1")
         self.layers = [PagedCache.empty(pages, kv_heads, head_dim, page, dtype, device) for _ in range(n_layers)]
         self.lens = torch.full((self.batch,), -1, dtype=torch.int32, device=device)
         self.host_lens = [-1] * self.batch

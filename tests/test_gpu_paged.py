@@ -535,3 +535,38 @@ def test_windows_of_any_size(new):
     v = cache.read(b)[1].expand(new, 2, 64) if new == 1 else cache.read(b)[1].expand(-1, 2, -1)
     assert torch.equal(own, v)
     assert torch.equal(cache.attend(b, q, window=1, sinks=2 ** 31 - 1), want)
+
+
+@pytest.mark.parametrize("new", [[1, 2], [20, 70]], ids=str)
+@pytest.mark.parametrize("form", [torch.float16, torch.int8], ids=["f16", "i8"])
+def test_positions_behind_every_table(form, new):
+    """Up to the largest that 32 bits hold: nothing is stored, zeros are read, and rows see what one at the table's last
+    position sees."""
+    before = _pages(form, 4, 2, 16, 64, 40)
+    cache = _cache(before)
+    table = torch.arange(4, dtype=torch.int32).view(2, 2)
+    pos = torch.tensor([2 ** 31 - 1 - new[0], 2 ** 31 - 1 - new[1] // 2], dtype=torch.int32)
+    batch = cache.batch(new, pos.to(DEV), table.to(DEV))
+    k, v, q = (torch.randn(sum(new), 2, 64, generator=torch.Generator().manual_seed(41)).half() for _ in range(3))
+    cache.append(batch, k.to(DEV), v.to(DEV))
+    assert all(a is None or torch.equal(_bits(a), _bits(b)) for a, b in zip(_host(cache), before))
+    out = cache.read(batch, out=tuple(torch.full((sum(new), 2, 64), 5.0, device=DEV).half() for _ in range(2)))
+    assert not bool(out[0].any()) and not bool(out[1].any())
+    rows = table.repeat_interleave(torch.tensor(new), 0)
+    for window, sinks in ((0, 0), (9, 3), (40, 0)):
+        got = cache.attend(batch, q.to(DEV), window=window, sinks=sinks).cpu()
+        _check_attention(cache, before, [1] * sum(new), [31] * sum(new), rows, q, got, window, sinks)
+
+
+def test_what_does_not_belong_together_is_refused():
+    cache = _cache(_pages(torch.float16, 4, 2, 16, 64, 42))
+    batch = cache.batch([1], [0], torch.zeros(1, 1, dtype=torch.int32, device=DEV))
+    q = torch.zeros(1, 2, 64, dtype=torch.float16, device=DEV)
+    for window, sinks in ((-1, 0), (0, -1), (2 ** 31, 0), (2 ** 32 + 1, 0), (1, 2 ** 32)):
+        with pytest.raises(ValueError, match="window and sinks"):
+            cache.attend(batch, q, window=window, sinks=sinks)
+    cache.attend(batch, q, window=2 ** 31 - 1, sinks=2 ** 31 - 1)
+    batch.table = torch.zeros(1, 1, dtype=torch.int32)   # (as a batch made for pages elsewhere)
+    for call in (lambda: cache.append(batch, q, q), lambda: cache.read(batch), lambda: cache.attend(batch, q)):
+        with pytest.raises(ValueError, match="the batch is on"):
+            call()

@@ -61,7 +61,7 @@ BAD_CACHES = [dict(dtype=_capi.MSA_F32), dict(dtype=7), dict(format=3), dict(for
               dict(page=8), dict(page=48), dict(page=512), dict(page=0), dict(kv_heads=0), dict(pages=0), dict(k_pages=None),
               dict(v_pages=None), dict(k_pages=4100), dict(format=1), dict(format=2, k_exp=ONE),
               dict(format=2, k_exp=ONE, v_exp=4097)]
-BAD_BATCHES = [dict(M=-1), dict(nseq=-1), dict(max_count=-1), dict(key_bound=-1), dict(min_count=-1), dict(min_count=2), dict(blocks=0), dict(table_stride=15),
+BAD_BATCHES = [dict(M=-1), dict(M=1 << 24), dict(max_count=1 << 24), dict(nseq=-1), dict(max_count=-1), dict(key_bound=-1), dict(min_count=-1), dict(min_count=2), dict(blocks=0), dict(table_stride=15),
                dict(blocks=(1 << 24) + 1, table_stride=1 << 25), dict(nseq=(1 << 20) + 1), dict(seq_start=None), dict(seq_pos=None),
                dict(table=None)]
 BAD_ARGS = [dict(heads=0), dict(heads=6), dict(heads=-4), dict(q=None), dict(out=None), dict(q=4100), dict(out=4104),
