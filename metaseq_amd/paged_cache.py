@@ -140,22 +140,20 @@ class PagedCache:
         return self._c[dtype][1]
 
     def _rows(self, name, t, rows, heads, copy):
-        """``t`` as rows of heads, one behind the other, that the kernels can read or write in place."""
+        """``t`` as rows of heads, one behind the other, that the kernels can read or write in place: (tensor, address,
+        row stride)."""
         if t.shape != (rows, heads, self.head_dim) or t.device != self.device:
             raise ValueError("%s must be [%d, %d, %d] on %s, not %s on %s"
                              % (name, rows, heads, self.head_dim, self.device, list(t.shape), t.device))
         sr, sh, sd = t.stride()
-        if sd == 1 and (heads == 1 or sh == self.head_dim) and t.data_ptr() % 16 == 0 and \
-                (rows < 2 or (sr % 8 == 0 and sr >= heads * self.head_dim)):
-            return t
+        at, width = t.data_ptr(), heads * self.head_dim
+        if sd == 1 and (heads == 1 or sh == self.head_dim) and at % 16 == 0 and (rows < 2 or (sr % 8 == 0 and sr >= width)):
+            return t, at, sr if rows > 1 else width
         if not copy:
             raise ValueError("%s must have its heads one behind the other, 16-byte aligned, rows a multiple of 8 apart"
                              % name)
-        return t.contiguous() if not t.is_contiguous() else t.clone()
-
-    @staticmethod
-    def _ld(t):
-        return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+        t = t.contiguous() if not t.is_contiguous() else t.clone()
+        return t, t.data_ptr(), width
 
     def _run(self, fn, *args):
         at = self.device.index
@@ -174,9 +172,9 @@ class PagedCache:
         if k.dtype != v.dtype:
             raise ValueError("keys are %s, values %s" % (k.dtype, v.dtype))
         c = self._of(k.dtype, batch)
-        k = self._rows("k", k, batch.rows, self.kv_heads, True)
-        v = self._rows("v", v, batch.rows, self.kv_heads, True)
-        self._run(self._lib.msa_paged_append, c, batch.by_ref, k.data_ptr(), self._ld(k), v.data_ptr(), self._ld(v))
+        k, k_at, ldk = self._rows("k", k, batch.rows, self.kv_heads, True)
+        v, v_at, ldv = self._rows("v", v, batch.rows, self.kv_heads, True)
+        self._run(self._lib.msa_paged_append, c, batch.by_ref, k_at, ldk, v_at, ldv)
 
     def read(self, batch, dtype=None, out=None):
         """Keys and values at the positions of a batch's tokens, ([rows, kv_heads, head_dim],) * 2 of ``dtype`` (8-bit
@@ -189,8 +187,8 @@ class PagedCache:
         elif out[0].dtype != out[1].dtype or dtype not in (None, out[0].dtype):
             raise ValueError("keys and values come in one dtype")
         c = self._of(out[0].dtype, batch)
-        k, v = (self._rows("out", t, batch.rows, self.kv_heads, False) for t in out)
-        self._run(self._lib.msa_paged_read, c, batch.by_ref, k.data_ptr(), self._ld(k), v.data_ptr(), self._ld(v))
+        (_, k_at, ldk), (_, v_at, ldv) = (self._rows("out", t, batch.rows, self.kv_heads, False) for t in out)
+        self._run(self._lib.msa_paged_read, c, batch.by_ref, k_at, ldk, v_at, ldv)
         return out
 
     def attend(self, batch, q, *, scale=None, window=0, sinks=0, out=None):
@@ -204,14 +202,15 @@ class PagedCache:
             raise ValueError("window and sinks must be 0 .. 2^31 - 1")
         c = self._of(q.dtype, batch)
         heads = q.shape[1]
-        q = self._rows("q", q, batch.rows, heads, True)
+        q, q_at, ldq = self._rows("q", q, batch.rows, heads, True)
         if out is None:
             out = torch.empty(batch.rows, heads, self.head_dim, dtype=q.dtype, device=self.device)
+            out_at, ldo = out.data_ptr(), heads * self.head_dim
         elif out.dtype != q.dtype:
             raise ValueError("out must be %s" % q.dtype)
         else:
-            self._rows("out", out, batch.rows, heads, False)
-        a = _capi.PagedAttentionArgs(heads, q.data_ptr(), self._ld(q), out.data_ptr(), self._ld(out), 0, window, sinks,
+            _, out_at, ldo = self._rows("out", out, batch.rows, heads, False)
+        a = _capi.PagedAttentionArgs(heads, q_at, ldq, out_at, ldo, 0, window, sinks,
                                      self._scale if scale is None else scale, None, 0)
         ref = ctypes.byref(a)
         what = (self.kv_heads, self.head_dim, self.k_pages.dtype, heads, window, sinks)
