@@ -87,12 +87,14 @@ struct Plan {
   int tile_blocks, tile_splits, grouped;  // tile kernel (tile_blocks 0: not launched)
 };
 
-// Splits of the keys: none where there are 128 workgroups, otherwise up to about 256 (one a CU), of at least `least` tiles
-// each.  (us, attention and sum: 192 workgroups over 4112 keys 45 in one, 47 + 5 in two, 46 + 5 in five; 8 over 131072
-// 75 + 5 in 16, 51 + 5 in 32, 52 + 5 in 64, 54 + 6 in 128)
-int splits_of(int64_t groups, int64_t tiles, int64_t least) {
-  const int64_t most = (tiles + least - 1) / least;
-  int64_t s = groups >= 128 ? 1 : 256 / groups;
+// Splits of the keys, of at least PA_NW tiles each: up to 128 workgroups are made about 256 (one a CU); from there to 255, of
+// which some CUs would have two and others one, four each share better if they stay long; 256 and more are left alone.
+// (us, attention and sum in 1, 2, 4, 8 splits: 128 workgroups over 700 keys in fp16 15, 15, 15, 19, over 4000 68, 49, 50, 50, e4m3 39,
+// 29, 29, 32; 160 over 16000 264, 277, 204, 200; 192 272, 265, 233, 229, e4m3 134, 134, 129, 123, over 4112 45, 52, 51, 54; 256 e4m3
+// over 16000 158, 163, 160, 160; 1024 over 640 to 1281 98, 99, 101, 120; 8 over 131072 in int8 80 in 16, 56 in 32, 57 in 64, 60 in 128)
+int splits_of(int64_t groups, int64_t tiles) {
+  const int64_t most = (tiles + PA_NW - 1) / PA_NW;
+  int64_t s = groups <= 128 ? 256 / groups : groups < 256 && tiles >= 96 ? 4 : 1;
   if (s > most) s = most;
   if (s > 128) s = 128;
   return s < 1 ? 1 : (int)s;
@@ -126,7 +128,7 @@ Plan plan_of(const msa_paged_cache& c, const msa_paged_batch& b, const msa_paged
     p.row_blocks = (int)((most + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
     const int kt = c.format == MSA_PAGES_SAME ? 32 : 64;
     const int64_t units = (int64_t)b.nseq * p.row_blocks * c.kv_heads;
-    p.splits = splits_of(units, (keys_of(most) + kt - 1) / kt, PA_NW);
+    p.splits = splits_of(units, (keys_of(most) + kt - 1) / kt);
   }
   if (rows > few) {
     p.tile_blocks = (int)((rows + PT_BM - 1) / PT_BM);
