@@ -13,6 +13,13 @@
 // the matrix cores take, for fp16 scaled by 2^SHIFT so that they stay normal down to 2^-24 of the maximum.
 // 8 bits: a code is exact in fp16.  The key's exponent scales the score; the value's goes into the probability, relative to the
 // largest exponent E met so far (the accumulators are in units of 2^E), in fp32, before it is rounded.
+//
+// Bound by HBM: a key and value cost 4 hd (2 hd) bytes and 4 hd operations a row.  Measured, heads of 128, the read of all keys
+// and values, beside 7.0 TB/s of a plain read: 32 sequences of 648 to 1282 keys, 32 heads, fp16, 500 MB, 107 us, 4.7 TB/s
+// (256 such sequences 6.0: some 15 us are the start - position, page and keys, one after the other - and the end of
+// workgroups that all run at once); 64 sequences, 72 heads, e4m3, 1.07 GB, 190 us, 5.6 TB/s; one of 131072 keys, 8 heads,
+// int8, 273 MB, 50 us, 5.4 TB/s, and 5 us for the sum of 32 splits; one of 58 keys, 12 heads of 64, 4.6 us.  Tried without
+// gain: tiles of 64 keys of 16 bits (106 us instead of 108), one or two waves a unit, three waves a SIMD by fewer registers.
 #pragma once
 
 #include <math.h>
@@ -523,6 +530,14 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
 // 16-bit pages go to LDS directly (global_load_lds_dwordx4: 16 bytes a lane to consecutive places, from anywhere), 8-bit
 // ones through registers, where they become fp16: keys times 2^(e - the tile's largest e), values times 2^(e - E), E the largest so
 // far.  Chunks of 16 bytes of a row are exchanged by the row's number, so that reads of many rows meet all banks.
+//
+// Bound by the vector units beside the matrix cores: a wave's tile of 128 dimensions is 32 products of 32 cycles and, for
+// 32 scores a lane, as many exponentials (16 cycles each) and some 150 other instructions, and the two waves that a SIMD
+// holds overlap little of it.  Measured, heads of 128, beside 1.14 PFLOP/s of a large product: 8192 tokens of 32 heads from
+// the start, fp16, 550 GFLOP, 0.64 to 0.72 ms, 0.76 to 0.86 PFLOP/s; four portions of 304 to 513 tokens of 32 heads behind
+// 1101 to 1536, 39.5 GFLOP, 79 us, 0.50; bf16, portions of 4096 and 2324 tokens of 32 heads on 8 with a window of 1024,
+// 108 GFLOP, 180 us, 0.60 (tiles at the window's ends are computed whole).  Tried without gain: the scheduler's group
+// hints, wave priorities; without loads the kernel takes 0.9 of its time, without the product with V 0.87.
 constexpr int PT_BM = 128, PT_BN = 64, PT_THREADS = 256;
 
 typedef __attribute__((address_space(3))) void pt_lds_void;

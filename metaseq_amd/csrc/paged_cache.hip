@@ -63,7 +63,9 @@ __device__ __forceinline__ uint32_t code2(float x, float y) {
   return whole(x) | (whole(y) << 8);
 }
 
-// One wave per (row, key/value head): the form for few rows per sequence.
+// One wave per (row, key/value head): the form for few rows per sequence.  A call of these sizes is latency: where the row belongs,
+// its position, its page, then the row.  (Measured: one token of 12 heads of 64 bf16 to e4m3 3.6 us, a plain launch 2 to 3; 32 tokens
+// of 32 heads of 128 fp16, whose values are 131072 pieces of two bytes in lines of their own, 7.8 us)
 template <int DT, int F>
 __global__ __launch_bounds__(256) void append_rows_kernel(PagedRows a) {
   typedef typename Elem<DT>::T T;
@@ -130,6 +132,7 @@ __device__ __forceinline__ float value_of(uint8_t c) {
   return (float)(int8_t)c;
 }
 
+// The other way.  (One token of 12 heads of 64 from e4m3 3.0 us)
 template <int DT, int F>
 __global__ __launch_bounds__(256) void read_rows_kernel(PagedRows a) {
   typedef typename Elem<DT>::T T;
@@ -163,7 +166,11 @@ __global__ __launch_bounds__(256) void read_rows_kernel(PagedRows a) {
 
 // Workgroup = 64 consecutive positions (from a multiple of 64 on) of a sequence, one key/value head: the form for portions of
 // prompts.  Rows are read and written 16 bytes a lane; values cross over in LDS, and leave (or come) as 16 bytes of one
-// dimension's consecutive positions.  Bound by HBM.
+// dimension's consecutive positions.  Bound by HBM, 64 positions being a whole line of every dimension in 16 bits.  The heads
+// of a block are neighbours, as their pieces of a row are.  (Measured, heads of 128, beside
+// a copy's 5.2 TB/s: append of 5047 tokens of 32 heads fp16 to int8, 124 MB, 35 us, 3.5 TB/s, reading them back 23 us, 5.4; of
+// 56547 tokens of 8 heads bf16 to e4m3, 348 MB, 98 and 73 us; reading 25576 tokens of 32 heads as they are, 838 MB, 175 us,
+// 4.8 TB/s.  Appending in 8 bits waits for a row's largest value between its loads and its stores)
 constexpr int PB = 64;  // positions of a block
 // From this many new tokens of the longest sequence on the blocks are ahead of a wave for every row, which writes (or reads)
 // its values two bytes at a time.  (us, rows and blocks, 64 sequences of 72 heads of 128: fp16 append of 2 15 and 16, of 3 24
