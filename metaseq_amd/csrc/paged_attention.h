@@ -14,12 +14,13 @@
 // 8 bits: a code is exact in fp16.  The key's exponent scales the score; the value's goes into the probability, relative to the
 // largest exponent E met so far (the accumulators are in units of 2^E), in fp32, before it is rounded.
 //
-// Bound by HBM: a key and value cost 4 hd (2 hd) bytes and 4 hd operations a row.  Measured, heads of 128, the read of all keys
-// and values, beside 7.0 TB/s of a plain read: 32 sequences of 648 to 1282 keys, 32 heads, fp16, 500 MB, 107 us, 4.7 TB/s
-// (256 such sequences 6.0: some 15 us are the start - position, page and keys, one after the other - and the end of
-// workgroups that all run at once); 64 sequences, 72 heads, e4m3, 1.07 GB, 190 us, 5.6 TB/s; one of 131072 keys, 8 heads,
-// int8, 273 MB, 50 us, 5.4 TB/s, and 5 us for the sum of 32 splits; one of 58 keys, 12 heads of 64, 4.6 us.  Tried without
-// gain: tiles of 64 keys of 16 bits (106 us instead of 108), one or two waves a unit, three waves a SIMD by fewer registers.
+// Bound by HBM: a key and value cost 4 hd (2 hd) bytes and 4 hd operations a row.  Reads through the caches end at 5.9 to 6.1 TB/s
+// here, in pieces of 64 bytes a row or whole lines, in a kernel that does nothing else; whole lines past the caches at 6.7,
+// pieces of 64 bytes past them at 6.1, but an operand of the matrix cores is 64 bytes of sixteen rows.  Measured, heads of 128, all
+// keys and values: 64 sequences of 1280 keys, 32 heads, fp16, 1.34 GB, 221 us, 6.1 TB/s; 32 of 648 to 1282, 500 MB, 98 us, 5.1
+// (and 107 behind an append); 64 sequences, 72 heads, e4m3, 1.07 GB, 190 us, 5.6 TB/s; one of 131072 keys, 8 heads, int8,
+// 273 MB, 50 us, 5.4 TB/s, and 5 us for the sum of 32 splits; one of 58 keys, 12 heads of 64, 4.6 us.  Tried without gain: tiles
+// of 64 keys of 16 bits (106 us instead of 108), one or two waves a unit, two to four workgroups a CU.
 #pragma once
 
 #include <math.h>

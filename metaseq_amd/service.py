@@ -406,7 +406,8 @@ class ContinuousBatcher(_Front):
     of a logit, as they do between batches of the reference's own service.
 
     ``cache_args``: keyword arguments of the decoder's ``new_paged_cache`` (``dtype=torch.int8`` keeps keys and
-    values in 8 bits, ``page``, ``window``, ``sinks``): the slots then live in pages."""
+    values in 8 bits, ``page``, ``window``, ``sinks``): the slots then live in pages, enough for all of them at
+    their capacity (``pages`` may ask for more, not for less: a step must never be short of one)."""
 
     def __init__(self, interface, slots: int = 32, capacity: int = MAX_SEQ_LEN,
                  idle_ms: float = 2.0, noise_fn=None, patience: int = 64,
@@ -425,6 +426,12 @@ class ContinuousBatcher(_Front):
         self.batch = SlotBatch(slots, capacity)
         self.backlog = Backlog()
         self.cache = None  # allocated with the first request
+        if cache_args is not None:
+            if not hasattr(self.decoder, "new_paged_cache"):
+                raise ValueError("this decoder has no paged cache")
+            pages = cache_args.get("pages")
+            if pages is not None and pages < slots * -(-capacity // cache_args.get("page", 64)):
+                raise ValueError("%d pages do not hold %d slots of %d positions" % (pages, slots, capacity))
         self.cache_args = cache_args
         self._stop: tuple = ()  # stop ids of the running batch
         self.noise_fn, self.patience = noise_fn, int(patience)

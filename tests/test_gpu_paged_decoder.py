@@ -208,3 +208,13 @@ def test_continuous_batching_over_pages(form):
             z = want[len(p) + i]
             assert float(z.max() - z[tok]) <= 2 * (2e-2 + 2 * own), (i, tok)
     assert all(n == -1 for n in engine.cache.host_lens) and sorted(engine.cache.free) == list(range(16))
+
+
+def test_an_engine_is_refused_pages_that_a_step_could_run_out_of():
+    from metaseq_amd.service import ContinuousBatcher
+
+    cfg, _, model = _model()
+    api = GeneratorInterface(model, Dictionary(cfg.vocab_size))
+    with pytest.raises(ValueError, match="15 pages"):
+        ContinuousBatcher(api, slots=4, capacity=64, cache_args=dict(page=16, pages=15))
+    ContinuousBatcher(api, slots=4, capacity=64, cache_args=dict(page=16, pages=16))
