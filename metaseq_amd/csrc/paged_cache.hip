@@ -215,8 +215,11 @@ __device__ __forceinline__ pg_u2 quantise8(pg_u4 w, int& e) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) m2 = __builtin_elementwise_max(m2, __builtin_bit_cast(u16x2, w[j] & 0x7fff7fffu));
   uint32_t bits = max((uint32_t)m2[0], (uint32_t)m2[1]);
-#pragma unroll
-  for (int o = LR / 2; o > 0; o >>= 1) bits = max(bits, (uint32_t)__shfl_xor((int)bits, o, MSA_WAVE));
+  bits = max(bits, (uint32_t)__builtin_amdgcn_mov_dpp((int)bits, 0xB1, 0xf, 0xf, true));   // the lane next door, the pair
+  bits = max(bits, (uint32_t)__builtin_amdgcn_mov_dpp((int)bits, 0x4E, 0xf, 0xf, true));   // next door, the other half of eight
+  bits = max(bits, (uint32_t)__builtin_amdgcn_mov_dpp((int)bits, 0x141, 0xf, 0xf, true));  // (mirrored), of sixteen
+  if (LR > 8) bits = max(bits, (uint32_t)__builtin_amdgcn_mov_dpp((int)bits, 0x140, 0xf, 0xf, true));
+  if (LR > 16) bits = max(bits, (uint32_t)__shfl_xor((int)bits, 16, MSA_WAVE));
   const float cap = largest<DT, F>();
   pg_u2 out;
   if (__ballot(bits > INF || of(bits) > cap)) {
