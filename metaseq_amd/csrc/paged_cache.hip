@@ -168,9 +168,9 @@ __global__ __launch_bounds__(256) void read_rows_kernel(PagedRows a) {
 // prompts.  Rows are read and written 16 bytes a lane; values cross over in LDS, and leave (or come) as 16 bytes of one
 // dimension's consecutive positions.  Bound by HBM, 64 positions being a whole line of every dimension in 16 bits.  The heads
 // of a block are neighbours, as their pieces of a row are.  (Measured, heads of 128, beside
-// a copy's 5.2 TB/s: append of 5047 tokens of 32 heads fp16 to int8, 124 MB, 35 us, 3.5 TB/s, reading them back 23 us, 5.4; of
-// 56547 tokens of 8 heads bf16 to e4m3, 348 MB, 98 and 73 us; reading 25576 tokens of 32 heads as they are, 838 MB, 175 us,
-// 4.8 TB/s.  Appending in 8 bits waits for a row's largest value between its loads and its stores)
+// a copy's 5.2 TB/s: append of 5047 tokens of 32 heads fp16 to int8, 124 MB, 32 us, 3.9 TB/s, reading them back 22 us, 5.7; of
+// 56547 tokens of 8 heads bf16 to e4m3, 348 MB, 82 us, 4.2, and 53 us, 6.6 with part of the pages still cached; reading 25576 tokens
+// of 32 heads as they are, 838 MB, 161 us, 5.2.  Appending in 8 bits waits for a row's largest value between loads and stores)
 constexpr int PB = 64;  // positions of a block
 // From this many new tokens of the longest sequence on the blocks are ahead of a wave for every row, which writes (or reads)
 // its values two bytes at a time.  (us, rows and blocks, 64 sequences of 72 heads of 128: fp16 append of 2 15 and 16, of 3 24
@@ -261,7 +261,19 @@ __device__ __forceinline__ pg_u2 quantise8(pg_u4 w, int& e) {
   return out;
 }
 
-template <int DT, int F, int HD>
+// Rows that are read or written once, in whole lines: NT past the caches.
+template <bool NT, typename W>
+__device__ __forceinline__ W load_once(const void* p) {
+  if (NT) return __builtin_nontemporal_load((const W*)p);
+  return *(const W*)p;
+}
+template <bool NT>
+__device__ __forceinline__ void store_once(void* p, pg_u4 w) {
+  if (NT) __builtin_nontemporal_store(w, (pg_u4*)p);
+  else *(pg_u4*)p = w;
+}
+
+template <int DT, int F, int HD, bool NT>
 __global__ __launch_bounds__(256) void append_block_kernel(PagedRows a, int blocks) {
   typedef typename Elem<DT>::T T;
   constexpr int ES = F < PG_E4M3 ? 2 : 1, LR = row_lanes<HD>(), RP = 256 / LR, N = PB / RP;
@@ -281,8 +293,8 @@ __global__ __launch_bounds__(256) void append_block_kernel(PagedRows a, int bloc
     k[i] = v[i] = pg_u4{0, 0, 0, 0};
     if (p >= b.begin && p < b.end && lane * 8 < HD) {
       const int64_t row = b.row + r0 + i * RP;
-      k[i] = *(const pg_u4*)((const T*)a.k + row * a.ldk + h * HD + lane * 8);
-      v[i] = *(const pg_u4*)((const T*)a.v + row * a.ldv + h * HD + lane * 8);
+      k[i] = load_once<NT, pg_u4>((const T*)a.k + row * a.ldk + h * HD + lane * 8);
+      v[i] = load_once<NT, pg_u4>((const T*)a.v + row * a.ldv + h * HD + lane * 8);
     }
   }
 #pragma unroll
@@ -352,7 +364,7 @@ __global__ __launch_bounds__(256) void append_block_kernel(PagedRows a, int bloc
   }
 }
 
-template <int DT, int F, int HD>
+template <int DT, int F, int HD, bool NT>
 __global__ __launch_bounds__(256) void read_block_kernel(PagedRows a, int blocks) {
   typedef typename Elem<DT>::T T;
   constexpr int ES = F < PG_E4M3 ? 2 : 1, LR = row_lanes<HD>(), RP = 256 / LR, N = PB / RP;
@@ -383,7 +395,7 @@ __global__ __launch_bounds__(256) void read_block_kernel(PagedRows a, int blocks
     const int at = threadIdx.x + i * 256, d = at / NG, p = b.first + (at % NG) * G;
     v[i] = pg_u4{0, 0, 0, 0};
     const int pg = at < HD * NG && p + G > b.begin && p < b.end ? page_of(a, s, p) : -1;
-    if (pg >= 0) v[i] = *(const pg_u4*)((const char*)a.c.v_pages + ((((int64_t)pg * a.c.kv_heads + h) * HD + d) * page + (p & (page - 1))) * ES);
+    if (pg >= 0) v[i] = load_once<NT, pg_u4>((const char*)a.c.v_pages + ((((int64_t)pg * a.c.kv_heads + h) * HD + d) * page + (p & (page - 1))) * ES);
   }
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -394,9 +406,9 @@ __global__ __launch_bounds__(256) void read_block_kernel(PagedRows a, int blocks
     ke[i] = ve[i] = 0;
     if (pg >= 0 && lane * 8 < HD) {
       if (ES == 2) {
-        k[i] = *(const pg_u4*)((const T*)a.c.k_pages + place * HD + lane * 8);
+        k[i] = load_once<NT, pg_u4>((const T*)a.c.k_pages + place * HD + lane * 8);
       } else {
-        const pg_u2 w = *(const pg_u2*)((const uint8_t*)a.c.k_pages + place * HD + lane * 8);
+        const pg_u2 w = load_once<NT, pg_u2>((const uint8_t*)a.c.k_pages + place * HD + lane * 8);
         k[i][0] = w[0], k[i][1] = w[1];
         ke[i] = a.c.k_exp[place], ve[i] = a.c.v_exp[place];
       }
@@ -417,7 +429,7 @@ __global__ __launch_bounds__(256) void read_block_kernel(PagedRows a, int blocks
   for (int i = 0; i < N; ++i) {
     const int p = b.first + r0 + i * RP;
     if (p >= b.begin && p < b.end && lane * 8 < HD)
-      *(pg_u4*)((T*)a.k_out + (int64_t)(b.row + r0 + i * RP) * a.ldk + h * HD + lane * 8) = rows_of(k[i], ke[i]);
+      store_once<NT>((T*)a.k_out + (int64_t)(b.row + r0 + i * RP) * a.ldk + h * HD + lane * 8, rows_of(k[i], ke[i]));
   }
   __syncthreads();
 #pragma unroll
@@ -428,7 +440,7 @@ __global__ __launch_bounds__(256) void read_block_kernel(PagedRows a, int blocks
     pg_u4 w = {0, 0, 0, 0};
 #pragma unroll
     for (int j = 0; j < 2 * ES; ++j) w[j] = *(const uint32_t*)(from + j * 4);
-    *(pg_u4*)((T*)a.v_out + (int64_t)(b.row + r0 + i * RP) * a.ldv + h * HD + lane * 8) = rows_of(w, ve[i]);
+    store_once<NT>((T*)a.v_out + (int64_t)(b.row + r0 + i * RP) * a.ldv + h * HD + lane * 8, rows_of(w, ve[i]));
   }
 }
 
@@ -442,8 +454,24 @@ void launch_rows_hd(const PagedRows& a, bool append, hipStream_t s) {
   }
   const int blocks = (a.b.max_count + PB - 2) / PB + 1;  // that max_count positions can meet
   const dim3 grid((unsigned)((int64_t)a.b.nseq * blocks * a.c.kv_heads));
-  if (append) hipLaunchKernelGGL((append_block_kernel<DT, F, HD>), grid, dim3(256), 0, s, a, blocks);
-  else hipLaunchKernelGGL((read_block_kernel<DT, F, HD>), grid, dim3(256), 0, s, a, blocks);
+  // Rows of 64 MB and more go past the caches, which the last and the next call could not find them in anyhow (us, through
+  // them and past them: read of 8 heads of 128 fp16, 40 MB 14 and 20, 77 MB 38 and 35, 315 MB 134 and 124; of 32 heads from e4m3,
+  // 30 MB 12 and 14, 122 MB 46 and 41; append to e4m3, 30 MB 13 and 14, 122 MB 48 and 44; append as they are, 315 MB 140 and 146:
+  // never).  Pages are written through the caches: attention reads them next.
+  const bool once = (int64_t)a.b.M * a.c.kv_heads * HD * 4 >= 64 << 20;
+  if (append) {
+    if constexpr (F >= PG_E4M3) {
+      if (once) {
+        hipLaunchKernelGGL((append_block_kernel<DT, F, HD, true>), grid, dim3(256), 0, s, a, blocks);
+        return;
+      }
+    }
+    hipLaunchKernelGGL((append_block_kernel<DT, F, HD, false>), grid, dim3(256), 0, s, a, blocks);
+  } else if (once) {
+    hipLaunchKernelGGL((read_block_kernel<DT, F, HD, true>), grid, dim3(256), 0, s, a, blocks);
+  } else {
+    hipLaunchKernelGGL((read_block_kernel<DT, F, HD, false>), grid, dim3(256), 0, s, a, blocks);
+  }
 }
 
 template <int DT, int F>

@@ -570,3 +570,24 @@ def test_what_does_not_belong_together_is_refused():
     for call in (lambda: cache.append(batch, q, q), lambda: cache.read(batch), lambda: cache.attend(batch, q)):
         with pytest.raises(ValueError, match="the batch is on"):
             call()
+
+
+@pytest.mark.parametrize("form", [torch.float16, E4M3, torch.int8], ids=["f16", "e4m3", "i8"])
+def test_a_call_of_many_rows_stores_and_reads_what_small_ones_do(form):
+    """More than 64 MB of rows, which go past the caches: pages and rows to the last bit those of calls of one sequence."""
+    seqs, n, heads, hd, page = 9, 510, 32, 128, 64
+    g = torch.Generator(device=DEV).manual_seed(50)
+    k, v = (torch.randn(seqs * n, heads, hd, generator=g, device=DEV).half() for _ in range(2))
+    table = torch.randperm(seqs * 8, generator=g, device=DEV).int().view(seqs, 8)
+    got = []
+    for each in (seqs, 1):
+        cache = _cache(_pages(form, seqs * 8, heads, page, hd, 51))
+        rows = []
+        for s in range(0, seqs, each):
+            batch = cache.batch([n] * each, [0 if i % 2 else 2 for i in range(s, s + each)], table[s:s + each])
+            part = slice(s * n, (s + each) * n)
+            cache.append(batch, k[part], v[part])
+            rows.append(cache.read(batch))
+        got.append(_host(cache) + [torch.cat([r[i] for r in rows]).cpu() for i in range(2)])
+    for a, b in zip(*got):
+        assert a is None or torch.equal(_bits(a), _bits(b))
