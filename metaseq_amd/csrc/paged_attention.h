@@ -23,6 +23,7 @@
 // of 64 keys of 16 bits (106 us instead of 108), one or two waves a unit, two to four workgroups a CU.
 #pragma once
 
+#include <float.h>
 #include <math.h>
 
 #include <atomic>
@@ -839,7 +840,9 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
     }
     // (a wave whose rows see nothing of the tile has nothing to do)
     const bool none = key0 > p_hi || w0 >= rows || (a.window > 0 && key0 + PT_BN - 1 <= p_lo - a.window && key0 >= a.sinks);
-    const float c = B8 ? ldexpf(qs, ek) : qs;
+    // (zeros have the least exponent there is, queries of zeros too: below what fp32 can be any score is zero, but those of keys
+    // that are not seen are -infinity, which a factor of zero would make NaN; above it a product of zero stays one)
+    const float c = B8 ? fminf(fmaxf(ldexpf(qs, ek), FLT_MIN), FLT_MAX) : qs;
     // Two copies: tiles that every row of the wave sees whole, and others.
     auto attend = [&](auto edge) {
       constexpr bool EDGE = decltype(edge)::value;

@@ -1,0 +1,99 @@
+"""Attention over 8-bit pages whose exponents are far apart, keys and queries of zeros, and what a row sees of others' tokens,
+against the definition in 64 bits.
+
+Tolerances are those of the attention's other tests, except that what is small is measured by what the row itself sees: with
+u = 2^-11 (probabilities in fp16), r the output's half step, w the softmax, A = sum_j w_j |v_j|, T = max_j w_j max_d |v_jd|:
+  r |o| + smallest subnormal / 2     the output's rounding
+  u A                                the rounding of every p_j
+  2 d A                              scores off by d = (hd + 8) 2^-24 max_j sum_i |q_i k_ij| scale, and 2^-16 for the addition of an
+                                     exponent (|z + e| 2^-24 with |e| < 2^7 and |z| < 2^7 where p_j counts); keys without weight
+                                     (below 2^-200) stay without it, and a lone key has a probability of one whatever its score
+  (n / 16 + 64) 2^-23 A              fp32 sums of n keys
+  n 2^-20 T                          probabilities below fp16's normal range: off by 2^-34 of the largest at most, times a value that is at
+                                     most 2^14 times that of the largest (2^12 of exponents and 2^2 of codes, where exponents are
+                                     left to the values; elsewhere they are part of the probabilities)
+"""
+import math
+
+import pytest
+import torch
+
+from oracle import paged_oracle as O
+from test_gpu_paged import _cache, _host, _pages, _table
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+E4M3 = torch.float8_e4m3fn
+FORMS = [(torch.float16, E4M3), (torch.bfloat16, E4M3), (torch.float16, torch.int8), (torch.bfloat16, torch.int8)]
+IDS = ["f16-e4m3", "bf16-e4m3", "f16-i8", "bf16-i8"]
+
+
+def _check(host, table, q, p, out, window=0, sinks=0):
+    """Rows q [n, heads, hd] of one sequence, at positions p .., against ``out``."""
+    n, heads, hd = q.shape
+    scale = 1.0 / math.sqrt(hd)
+    keys, there = O.positions(host[0], host[2], table, p + n, False)
+    values, _ = O.positions(host[1], host[3], table, p + n, True)
+    i, j = p + torch.arange(n)[:, None], torch.arange(p + n)[None]
+    see = (j <= i) & there
+    if window:
+        see &= (j > i - window) | (j < sinks)
+    keys[~see.any(0)] = values[~see.any(0)] = 0.0
+    group = heads // keys.shape[1]
+    k, v = (x.repeat_interleave(group, 1).transpose(0, 1) for x in (keys, values))   # [heads, positions, hd]
+    x = q.double().transpose(0, 1)
+    z = (x @ k.mT * scale).masked_fill(~see, -math.inf)
+    w = torch.nan_to_num(torch.softmax(z, -1))
+    want, weight, most = w @ v, w @ v.abs(), (w * v.abs().amax(-1).unsqueeze(1)).amax(-1, keepdim=True)
+    counts = w > 2.0 ** -200
+    size = (x.abs() @ k.abs().mT * scale * counts).amax(-1, keepdim=True) * (counts.sum(-1, keepdim=True) > 1)
+    d = (hd + 8) * 2.0 ** -24 * size + 2.0 ** -16
+    f = torch.finfo(q.dtype)
+    tol = f.eps / 2 * (want.abs() + f.smallest_normal) + (2.0 ** -11 + 2 * d + ((p + n) / 16 + 64) * 2.0 ** -23) * weight \
+        + (p + n) * 2.0 ** -20 * most
+    off = (out.double().transpose(0, 1) - want).abs()
+    bad = ~(off <= tol)
+    assert not bool(bad.any()), (int(bad.sum()), bad.nonzero()[0].tolist(), float((off / tol).nan_to_num(math.inf).max()))
+
+
+def _stored(form, dtype, k, v, page=16):
+    """A cache with one sequence's keys and values [positions, kv_heads, hd], and its table."""
+    n, kvh, hd = k.shape
+    blocks = -(-n // page)
+    cache = _cache(_pages(form, blocks + 1, kvh, page, hd, 3))
+    table = _table(1, [blocks], blocks + 1, 4)
+    cache.append(cache.batch([n], [0], table.to(DEV)), k.to(dtype).to(DEV), v.to(dtype).to(DEV))
+    return cache, table
+
+
+def _attend(cache, table, q, p, **kw):
+    return cache.attend(cache.batch([len(q)], [p], table.to(DEV)), q.to(DEV), **kw).cpu()
+
+
+@pytest.mark.parametrize("new", [1, 5, 70, 150])
+@pytest.mark.parametrize("dtype,form", FORMS, ids=IDS)
+def test_queries_and_keys_of_zeros(dtype, form, new):
+    """A row that likes no key better than another has the mean of the values it sees."""
+    g = torch.Generator().manual_seed(1)
+    p = 37
+    cache, table = _stored(form, dtype, torch.zeros(p + new, 1, 64), torch.randn(p + new, 1, 64, generator=g))
+    host = _host(cache)
+    assert bool((host[2].view(-1) == -126).any())
+    q = torch.randn(new, 2, 64, generator=g)
+    for size in (0.0, 2.0 ** -20, 2.0 ** -24) + ((2.0 ** -60, 2.0 ** -100) if dtype == torch.bfloat16 else ()):
+        rows = (q * size).to(dtype)
+        _check(host, table[0], rows, p, _attend(cache, table, rows, p))
+
+
+@pytest.mark.parametrize("new", [3, 150])
+@pytest.mark.parametrize("dtype,form", FORMS, ids=IDS)
+def test_rows_whose_first_pages_are_nowhere(dtype, form, new):
+    g = torch.Generator().manual_seed(2)
+    cache, table = _stored(form, dtype, torch.randn(250, 1, 64, generator=g), torch.randn(250, 1, 64, generator=g))
+    table[0, :6] = -1
+    p = 92
+    for size in (0.0, 2.0 ** -24, 1.0):
+        q = (torch.randn(new, 2, 64, generator=g) * size).to(dtype)
+        out = _attend(cache, table, q, p)
+        assert bool((out[:min(new, 4)] == 0).all())
+        _check(_host(cache), table[0], q, p, out)
