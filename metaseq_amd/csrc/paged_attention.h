@@ -142,6 +142,26 @@ __device__ __forceinline__ float pa_quads_sum(float v) {
   return v + __shfl_xor(v, 32, MSA_WAVE);
 }
 
+// Scores z_j c relative to the maximum m of them, in log2 units, as what exp2 takes is formed in one fused operation: z_j c - off.  The
+// maximum is a rounded product, which the fused operation's is not, and far from zero the two differ by more than exp2 can
+// take: there (from 2^16 on in some lane) z becomes the rounded products less the maximum, c one.  m = -infinity: no score yet.
+constexpr float PA_FAR = 65536.f;
+template <int N>
+__device__ __forceinline__ void pa_relative(float (&z)[N], float& c, float& off, float m, float shift) {
+#pragma clang fp contract(off)
+  const float from = m == -INFINITY ? 0.f : m;
+  off = from - shift;
+  if (__builtin_expect(__ballot(fabsf(from) >= PA_FAR) != 0, 0)) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float score = z[j] * c;
+      z[j] = score - from;
+    }
+    c = 1.f;
+    off = -shift;
+  }
+}
+
 // Of the N keys from `key` on (N <= 16), as bits, those that some row at a position between lo and hi sees (of
 // consecutive tokens; lo == hi: that the row sees).
 template <int N>
@@ -386,11 +406,12 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[rt][d][e] *= w;
       }
-      const float off = (m[rt] == -INFINITY ? 0.f : m[rt]) - (B8 ? 0.f : X::SHIFT);
+      float c = qs[rt], off;
+      pa_relative(z[rt], c, off, m[rt], B8 ? 0.f : X::SHIFT);
       float p[KQ], sum = 0.f;
 #pragma unroll
       for (int j = 0; j < KQ; ++j) {
-        p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[rt][j], qs[rt], -off));
+        p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[rt][j], c, -off));
         sum += p[j];
         if (B8) p[j] = ldexpf(p[j], ((seen >> j) & 1 ? byte_of(vx, j) : -127) - E + (int)X::SHIFT);
       }
@@ -714,19 +735,25 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
   // follow from them reach the lanes that need them through LDS of the wave's own.
   constexpr int CB = HD / 16, KN = (PT_BN * CB + PT_THREADS - 1) / PT_THREADS, VN = (HD * 4 + PT_THREADS - 1) / PT_THREADS;
   __shared__ __attribute__((aligned(16))) half_t s_factor[B8 ? PT_THREADS / 64 : 1][2][64];
+  // Addresses that follow from the thread's number are formed anew for each tile where registers end: kept across the loop they
+  // would take others to scratch memory.  (us, kept and formed anew: 256 dimensions, int8 230 and 134, e4m3, which has the
+  // registers, 125 and 129; 128 dimensions 111 and 115)
+  constexpr bool ANEW = F == PG_I8 && HD > 192;
   pg_u4 kr[B8 ? KN : 1], vr[B8 ? VN : 1];
   int ke = 0, ve = 0;
   const int vg = threadIdx.x & 3;       // the sixteen keys that the thread's chunks of V belong to
   auto fetch = [&](int i, PtPages pg) {
     const int key0 = tiles.tile(i) * PT_BN, in = page - 1;
+    int tid = threadIdx.x;
+    if (ANEW) asm volatile("" : "+v"(tid));
 #pragma unroll
     for (int j = 0; j < KN; ++j) {
-      const int at = min((int)threadIdx.x + j * PT_THREADS, PT_BN * CB - 1), row = at / CB, c = at % CB;
+      const int at = min(tid + j * PT_THREADS, PT_BN * CB - 1), row = at / CB, c = at % CB;
       kr[j] = *(const pg_u4*)((const char*)a.k_pages + h * unit + max(pg.of(row >> 4), 0) * page_bytes + ((key0 + row) & in) * HD + c * 16);
     }
     const char* from = (const char*)a.v_pages + h * unit + max(pg.of(vg), 0) * page_bytes + ((key0 + vg * 16) & in);
 #pragma unroll
-    for (int j = 0; j < VN; ++j) vr[j] = *(const pg_u4*)(from + (min((int)threadIdx.x + j * PT_THREADS, HD * 4 - 1) >> 2) * page);
+    for (int j = 0; j < VN; ++j) vr[j] = *(const pg_u4*)(from + (min(tid + j * PT_THREADS, HD * 4 - 1) >> 2) * page);
     const int64_t ul = ((int64_t)max(pg.of(lane >> 4), 0) * a.kv_heads + h) * page + ((key0 + lane) & in);
     ke = a.k_exp[ul];
     ve = a.v_exp[ul];
@@ -735,6 +762,8 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
   // (returns the exponents that the tile's keys and values are relative to)
   auto stage = [&](int i, int slot, PtPages pg, int& ek, int& ev) {
     const int key0 = tiles.tile(i) * PT_BN;
+    int tid = threadIdx.x;
+    if (ANEW) asm volatile("" : "+v"(tid));
     const bool mine = pg.of(lane >> 4) >= 0 && anyone(key0 + lane);
     ek = wave_most(mine ? ke : -127);
     ev = max(ev, wave_most(mine ? ve : -127));
@@ -746,7 +775,7 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
     char* vt = lds + (2 + slot) * TILEB;
 #pragma unroll
     for (int j = 0; j < KN; ++j) {
-      const int at = threadIdx.x + j * PT_THREADS, row = at / CB, c = at % CB;
+      const int at = tid + j * PT_THREADS, row = at / CB, c = at % CB;
       if ((PT_BN * CB) % PT_THREADS == 0 || at < PT_BN * CB) {
         const half_t f = s_factor[wave][0][row & 63];
 #pragma unroll
@@ -758,7 +787,7 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
     const uint32_t seen = pg.of(vg) >= 0 ? pa_seen<16>(key0 + vg * 16, g_lo, g_hi, a.window, a.sinks) : 0;
 #pragma unroll
     for (int j = 0; j < VN; ++j) {
-      const int at = threadIdx.x + j * PT_THREADS, row = at >> 2;
+      const int at = tid + j * PT_THREADS, row = at >> 2;
       if ((HD * 4) % PT_THREADS == 0 || at < HD * 4) {
         pg_u4 w = vr[j];
         if (seen != 0xffff) {
@@ -842,7 +871,7 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
     const bool none = key0 > p_hi || w0 >= rows || (a.window > 0 && key0 + PT_BN - 1 <= p_lo - a.window && key0 >= a.sinks);
     // (zeros have the least exponent there is, queries of zeros too: below what fp32 can be any score is zero, but those of keys
     // that are not seen are -infinity, which a factor of zero would make NaN; above it a product of zero stays one)
-    const float c = B8 ? fminf(fmaxf(ldexpf(qs, ek), FLT_MIN), FLT_MAX) : qs;
+    const float to_score = B8 ? fminf(fmaxf(ldexpf(qs, ek), FLT_MIN), FLT_MAX) : qs;
     // Two copies: tiles that every row of the wave sees whole, and others.
     auto attend = [&](auto edge) {
       constexpr bool EDGE = decltype(edge)::value;
@@ -883,7 +912,7 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
       float top = z[0];
 #pragma unroll
       for (int j = 1; j < 32; ++j) top = fmaxf(top, z[j]);
-      top *= c;
+      top *= to_score;
       if (B8 && ev > E) {
 #pragma unroll
         for (int d = 0; d < DBLK; ++d)
@@ -901,7 +930,8 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
 #pragma unroll
           for (int v = 0; v < 16; ++v) o[d][v] *= w;
       }
-      const float off = (m == -INFINITY ? 0.f : m) - SHIFT;
+      float c = to_score, off;
+      pa_relative(z, c, off, m, SHIFT);
       pg_u4 p[4];  // steps of sixteen keys of the product with V
       float sum[2] = {0.f, 0.f};  // of the probabilities as they are rounded
       auto pair = [&](int st, int j) {

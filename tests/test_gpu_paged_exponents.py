@@ -97,3 +97,33 @@ def test_rows_whose_first_pages_are_nowhere(dtype, form, new):
         out = _attend(cache, table, q, p)
         assert bool((out[:min(new, 4)] == 0).all())
         _check(_host(cache), table[0], q, p, out)
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("new,p", [(1, 60), (5, 60), (40, 60), (150, 60), (2, 3000), (130, 3000)])
+@pytest.mark.parametrize("dtype,form", [(torch.float16,) * 2, (torch.bfloat16,) * 2] + FORMS, ids=["f16", "bf16"] + IDS)
+def test_scores_of_any_size(dtype, form, new, p, sign):
+    """Products up to the largest that two numbers of the type have, every one of them exact: the row has the mean of the
+    values whose score is the largest, positive or negative."""
+    n, hd = p + new, 64
+    k = torch.zeros(n, 1, hd)
+    at = torch.arange(n)
+    k[at, 0, at % 4] = (1.0 if sign < 0 else 1.0 - 2.0 * (at // 4 % 2).float()) * 2.0 ** (15 if dtype == torch.float16 else 60)
+    v = torch.randn(n, 1, hd, generator=torch.Generator().manual_seed(9))
+    q = torch.zeros(new, 2, hd)
+    q[:, :, :4] = sign * torch.tensor([1.0, 2.0, 3.0, 5.0]) * 2.0 ** (13 if dtype == torch.float16 else 40)
+    best = k[:, 0, 3] > 0 if sign > 0 else k[:, 0, 0] > 0
+    if form == dtype:
+        cache, table = _cache(_pages(form, -(-n // 16), 1, 16, hd, 3)), torch.arange(-(-n // 16), dtype=torch.int32)[None]
+        cache.append(cache.batch([n], [0], table.to(DEV)), k.to(dtype).to(DEV), v.to(dtype).to(DEV))
+    else:
+        cache, table = _stored(form, dtype, k, v)
+    out = _attend(cache, table, q.to(dtype), p).double()
+    host = _host(cache)
+    values, _ = O.positions(host[1], host[3], table[0], n, True)
+    u = 2.0 ** -8 if form == torch.bfloat16 else 2.0 ** -11
+    for i in range(new):
+        seen = values[:p + i + 1][best[:p + i + 1], 0]
+        want, weight = seen.mean(0), seen.abs().mean(0)
+        tol = torch.finfo(dtype).eps / 2 * want.abs() + (u + (n / 16 + 64) * 2.0 ** -23) * weight
+        assert bool(((out[i] - want).abs() <= tol).all()), i
