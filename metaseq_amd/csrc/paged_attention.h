@@ -228,7 +228,8 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
 
   // ---- queries: B operand, row n16 of row tile rt, the dimensions that the lane's loads of K have ----
   pg_u4 qf[RT][KL][HALVES];
-  float qs[RT];  // what turns a product into a score in log2 units
+  const float qs = a.scale * PA_LOG2E;  // what turns a product into a score in log2 units
+  int eq[RT];    // 8 bits: the power of two that the row's queries stand for
   int pn[RT];    // the row's position; rows past the last one see nothing
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
@@ -237,7 +238,7 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
     const int t = live ? rho / group : 0, g = live ? rho - t * group : 0;
     pn[rt] = live ? (int)min((int64_t)pos + t, (int64_t)limit) : -1;
     const char* q = (const char*)a.q + (((int64_t)row0 + t) * a.ldq + (int64_t)(h * group + g) * HD) * 2;
-    qs[rt] = a.scale * PA_LOG2E;
+    eq[rt] = 0;
 #pragma unroll
     for (int c = 0; c < KL; ++c)
 #pragma unroll
@@ -267,7 +268,7 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
           for (int i = 0; i < 8; ++i) w[i] = (half_t)ldexpf((float)v[i], -k);
           qf[rt][c][e] = __builtin_bit_cast(pg_u4, w);
         }
-      qs[rt] = ldexpf(qs[rt], k);
+      eq[rt] = k;
     }
   }
 
@@ -391,11 +392,11 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
       float top = -INFINITY;
 #pragma unroll
       for (int j = 0; j < KQ; ++j) {
-        if (B8) z[rt][j] = ldexpf(z[rt][j], byte_of(kx, j));
+        if (B8) z[rt][j] = ldexpf(z[rt][j], byte_of(kx, j) + eq[rt]);  // (either alone may pass what fp32 holds)
         z[rt][j] = (sees >> j) & 1 ? z[rt][j] : -INFINITY;
         top = fmaxf(top, z[rt][j]);
       }
-      top *= qs[rt];
+      top *= qs;
       if (__ballot(top > m[rt] + PA_LAZY)) {  // (m = -inf: any score)
         const float to = fmaxf(m[rt], pa_quads_max(top));
         const float w = m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rt] - to);
@@ -406,7 +407,7 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[rt][d][e] *= w;
       }
-      float c = qs[rt], off;
+      float c = qs, off;
       pa_relative(z[rt], c, off, m[rt], B8 ? 0.f : X::SHIFT);
       float p[KQ], sum = 0.f;
 #pragma unroll

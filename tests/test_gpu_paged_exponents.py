@@ -127,3 +127,27 @@ def test_scores_of_any_size(dtype, form, new, p, sign):
         want, weight = seen.mean(0), seen.abs().mean(0)
         tol = torch.finfo(dtype).eps / 2 * want.abs() + (u + (n / 16 + 64) * 2.0 ** -23) * weight
         assert bool(((out[i] - want).abs() <= tol).all()), i
+
+
+def _with_infinities(dtype, form, new, p, sign, at, key, value):
+    g = torch.Generator().manual_seed(5)
+    k, v = (torch.randn(p + new, 1, 64, generator=g) for _ in range(2))
+    if key:
+        k[at, 0, 7] = math.inf
+    if value:
+        v[at, 0, 9] = -math.inf
+    q = torch.randn(new, 2, 64, generator=g)
+    q[:, :, 7] = sign * 2.0 ** (-9 if dtype == torch.bfloat16 else -4)
+    cache, table = _stored(form, dtype, k, v)
+    q = q.to(dtype)
+    _check(_host(cache), table[0], q, p, _attend(cache, table, q, p))
+
+
+@pytest.mark.parametrize("where", ["last", "first"])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("new", [1, 5])
+@pytest.mark.parametrize("dtype,form", FORMS, ids=IDS)
+def test_a_key_that_overflowed(dtype, form, new, sign, where):
+    """It is held as the largest that codes can stand for.  Queries that are small and positive in its place look at nothing
+    else, negative ones not at it; rows in front of it do not see it."""
+    _with_infinities(dtype, form, new, 60, sign, 60 + new - 1 if where == "last" else 33, True, False)
