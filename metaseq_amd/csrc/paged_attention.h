@@ -11,8 +11,11 @@
 // Softmax: running maximum m per row, in log2 units, taken over the quads only when a score passes it by more than
 // LAZY (probabilities then reach 2^LAZY at most); sums are fp32.  Probabilities are rounded to the 16-bit format that
 // the matrix cores take, for fp16 scaled by 2^SHIFT so that they stay normal down to 2^-24 of the maximum.
-// 8 bits: a code is exact in fp16.  The key's exponent scales the score; the value's goes into the probability, relative to the
-// largest exponent E met so far (the accumulators are in units of 2^E), in fp32, before it is rounded.
+// 8 bits: a code is exact in fp16.  The key's exponent scales the score; the value's, e, is added to the score, so that what is
+// rounded for the product with V is 2^(z - m + e - R), R the row's running maximum of z - m + e: the accumulators are in units of
+// 2^(m + R), and neither what other rows see nor a large value without weight takes anything from the row's own.  A second
+// exponential for each key hides behind the reads (64 sequences of 72 heads 191 us with it, 191 with one exponent for all
+// rows).
 //
 // Bound by HBM: a key and value cost 4 hd (2 hd) bytes and 4 hd operations a row.  Reads through the caches end at 5.9 to 6.1 TB/s
 // here, in pieces of 64 bytes a row or whole lines, in a kernel that does nothing else; whole lines past the caches at 6.7,
@@ -133,6 +136,12 @@ __device__ __forceinline__ uint32_t pa_finite(uint32_t w) {
   return out;
 }
 
+// x 2^e: the power alone may pass what fp32 holds
+__device__ __forceinline__ float pa_times_power(float x, float e) {
+  const float whole = floorf(e);
+  return ldexpf(x * __builtin_amdgcn_exp2f(e - whole), (int)fminf(fmaxf(whole, -1000.f), 1000.f));
+}
+
 __device__ __forceinline__ float pa_quads_max(float v) {
   v = fmaxf(v, __shfl_xor(v, 16, MSA_WAVE));
   return fmaxf(v, __shfl_xor(v, 32, MSA_WAVE));
@@ -206,7 +215,7 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
   constexpr int LDO = HD + 4;
   __shared__ __attribute__((aligned(16))) float s_acc[PA_NW][16][LDO];
   static_assert(16 * LDO * 4 >= HD * KT * ES, "a tile's values of one wave");
-  __shared__ float s_m[PA_NW][16], s_l[PA_NW][16];
+  __shared__ float s_m[PA_NW][16], s_l[PA_NW][16], s_r[B8 ? PA_NW : 1][16];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n16 = lane & 15, quad = lane >> 4;
@@ -273,15 +282,14 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
   }
 
   float4_t acc[RT][DT];
-  float m[RT], l[RT];
+  float m[RT], l[RT], R[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    m[rt] = -INFINITY;
+    m[rt] = R[rt] = -INFINITY;
     l[rt] = 0.f;
 #pragma unroll
     for (int d = 0; d < DT; ++d) acc[rt][d] = float4_t{0.f, 0.f, 0.f, 0.f};
   }
-  int E = -127;  // largest exponent of values met (8 bits)
 
   // ---- tiles.  As a source of K a lane has keys of quad n16 / 4, as one of V of its own quad.  Keys and values are
   // requested a tile ahead, each into the registers that the matrix instructions have just read.  (Nothing past the caches: a
@@ -348,23 +356,6 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
                        (pg.a | pg.b | pg.c | pg.d) >= 0;
     // the quad's keys that some row sees
     const uint32_t seen = whole ? ~0u : there ? pa_seen<KQ>(kq, p_lo, p_hi, a.window, a.sinks) : 0;
-    if (B8) {
-      int most = -127;
-#pragma unroll
-      for (int j = 0; j < KQ; ++j) most = max(most, (seen >> j) & 1 ? byte_of(vx, j) : -127);
-      if (__ballot(most > E)) {
-        most = max(most, __shfl_xor(most, 16, MSA_WAVE));
-        most = max(most, __shfl_xor(most, 32, MSA_WAVE));
-        const int to = max(E, __builtin_amdgcn_readfirstlane(most));
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[rt][d][e] = ldexpf(acc[rt][d][e], E - to);
-        E = to;
-      }
-    }
     float z[RT][KQ];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -400,23 +391,46 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
       if (__ballot(top > m[rt] + PA_LAZY)) {  // (m = -inf: any score)
         const float to = fmaxf(m[rt], pa_quads_max(top));
         const float w = m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rt] - to);
+        if (B8) {
+          R[rt] -= m[rt] == -INFINITY ? 0.f : to - m[rt];
+        } else {
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[rt][d][e] *= w;
+        }
         m[rt] = to;
         l[rt] *= w;
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[rt][d][e] *= w;
       }
       float c = qs, off;
       pa_relative(z[rt], c, off, m[rt], B8 ? 0.f : X::SHIFT);
       float p[KQ], sum = 0.f;
 #pragma unroll
       for (int j = 0; j < KQ; ++j) {
-        p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[rt][j], c, -off));
+        z[rt][j] = __builtin_fmaf(z[rt][j], c, -off);
+        p[j] = __builtin_amdgcn_exp2f(z[rt][j]);
         sum += p[j];
-        if (B8) p[j] = ldexpf(p[j], ((seen >> j) & 1 ? byte_of(vx, j) : -127) - E + (int)X::SHIFT);
       }
       l[rt] += sum;
+      if (B8) {
+        float most = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < KQ; ++j) {
+          z[rt][j] += (float)byte_of(vx, j);
+          most = fmaxf(most, z[rt][j]);
+        }
+        if (__ballot(most > R[rt] + PA_LAZY)) {
+          const float to = fmaxf(R[rt], pa_quads_max(most)), w = R[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(R[rt] - to);
+          R[rt] = to;
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[rt][d][e] *= w;
+        }
+        const float from = (R[rt] == -INFINITY ? 0.f : R[rt]) - X::SHIFT;
+#pragma unroll
+        for (int j = 0; j < KQ; ++j) p[j] = __builtin_amdgcn_exp2f(z[rt][j] - from);
+      }
 #pragma unroll
       for (int e = 0; e < HALVES; ++e) {
         if (F == PG_BF16) {
@@ -500,15 +514,13 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
     if (left <= 0) break;
     l[rt] = pa_quads_sum(l[rt]);
     if (rt > 0) __syncthreads();
-    if (quad == 0) s_m[wave][n16] = m[rt], s_l[wave][n16] = l[rt];
+    if (quad == 0) {
+      s_m[wave][n16] = m[rt], s_l[wave][n16] = l[rt];
+      if (B8) s_r[wave][n16] = R[rt] - X::SHIFT;
+    }
     if (n16 < left) {
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        float4_t v = acc[rt][d];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = B8 ? ldexpf(v[k], E - (int)X::SHIFT) : v[k];
-        *(float4_t*)&s_acc[wave][n16][d * 16 + quad * 4] = v;
-      }
+      for (int d = 0; d < DT; ++d) *(float4_t*)&s_acc[wave][n16][d * 16 + quad * 4] = acc[rt][d];
     }
     __syncthreads();
     for (int j = threadIdx.x; j < left * (HD / 4); j += PA_NW * 64) {
@@ -517,28 +529,36 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
 #pragma unroll
       for (int w = 0; w < PA_NW; ++w) to = fmaxf(to, s_m[w][r]);
       const float off = to == -INFINITY ? 0.f : to;
-      float total = 0.f;
+      float total = 0.f, unit = 0.f;  // (8 bits: o is in units of 2^unit)
+      if (B8) {
+        unit = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < PA_NW; ++w) unit = fmaxf(unit, s_m[w][r] - off + s_r[w][r]);
+        unit = unit == -INFINITY ? 0.f : unit;
+      }
       float4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < PA_NW; ++w) {
-        const float f = __builtin_amdgcn_exp2f(s_m[w][r] - off);
+        const float f = __builtin_amdgcn_exp2f(s_m[w][r] - off), g = B8 ? __builtin_amdgcn_exp2f(s_m[w][r] - off + s_r[w][r] - unit) : f;
         total += f * s_l[w][r];
         const float4_t v = *(const float4_t*)&s_acc[w][r][d];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o[k] += f * v[k];
+        for (int k = 0; k < 4; ++k) o[k] += g * v[k];
       }
       const int rho = rho0 + rt * 16 + r, t = rho / group, head = h * group + rho - t * group;
       const int64_t row = (int64_t)row0 + t;
       if (a.splits > 1) {
         float* part = a.partial + ((row * a.heads + head) * a.splits + split) * (HD + 4);
         *(float4_t*)(part + d) = o;
-        if (d == 0) part[HD] = to, part[HD + 1] = total;
+        if (d == 0) part[HD] = to, part[HD + 1] = total, part[HD + 2] = unit;
       } else {
         const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
         uint16_t w[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          w[k] = a.bf16 ? __builtin_bit_cast(uint16_t, (bf16_t)(o[k] * inv)) : __builtin_bit_cast(uint16_t, (half_t)(o[k] * inv));
+        for (int k = 0; k < 4; ++k) {
+          const float x = B8 ? pa_times_power(o[k] * inv, unit) : o[k] * inv;
+          w[k] = a.bf16 ? __builtin_bit_cast(uint16_t, (bf16_t)x) : __builtin_bit_cast(uint16_t, (half_t)x);
+        }
         const int64_t at = a.out_mb > 0 ? packed_act_offset((int)row, head * HD + d, a.out_mb) : row * a.ldo + head * HD + d;
         *(pg_u2*)((uint16_t*)a.out + at) = pg_u2{(uint32_t)w[0] | (uint32_t)w[1] << 16, (uint32_t)w[2] | (uint32_t)w[3] << 16};
       }
@@ -1017,7 +1037,7 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
         for (int r = 0; r < 4; ++r) v[r] = B8 ? ldexpf(o[db][blk * 4 + r], E) : o[db][blk * 4 + r];
         if (HD % 32 == 0 || d < HD) *(float4_t*)(to + d) = v;
       }
-    if (hl == 0) to[HD] = m, to[HD + 1] = l;
+    if (hl == 0) to[HD] = m, to[HD + 1] = l, to[HD + 2] = 0.f;
     return;
   }
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;

@@ -23,6 +23,7 @@ __global__ __launch_bounds__(PC_THREADS) void paged_combine_kernel(PagedAttentio
   __shared__ __attribute__((aligned(16))) float s_o[MANY ? PC_THREADS : 1][4];
   __shared__ float s_l[MANY ? PC_THREADS : 1];
   const int lane = threadIdx.x & 63, splits = a.splits;
+  const bool eight = a.k_exp != nullptr;
   const int s = tokens > 0 ? blockIdx.x / tokens : __builtin_amdgcn_readfirstlane(paged_sequence_of(a.seq_start, a.nseq, blockIdx.x));
   if (s >= a.nseq) return;
   const int row0 = a.seq_start[s], r = tokens > 0 ? row0 + (int)blockIdx.x - s * tokens : (int)blockIdx.x;
@@ -42,16 +43,29 @@ __global__ __launch_bounds__(PC_THREADS) void paged_combine_kernel(PagedAttentio
     for (int i = 0; i < splits; ++i) top = fmaxf(top, part[i * stride + hd]);
   }
   const float off = top == -INFINITY ? 0.f : top;
+  float unit = 0.f;  // of the sum, relative to the maximum
+  if (eight) {
+    unit = -INFINITY;
+    if constexpr (MANY) {
+      for (int i = lane; i < splits; i += 64) unit = fmaxf(unit, part[i * stride + hd] - off + part[i * stride + hd + 2]);
+      unit = wave_max(unit);
+    } else {
+#pragma unroll 4
+      for (int i = 0; i < splits; ++i) unit = fmaxf(unit, part[i * stride + hd] - off + part[i * stride + hd + 2]);
+    }
+    unit = unit == -INFINITY ? 0.f : unit;
+  }
   float4_t o = {0.f, 0.f, 0.f, 0.f};
   float total = 0.f;
   if (g < groups) {
 #pragma unroll 4
     for (int i = MANY ? g : 0; i < splits; i += MANY ? groups : 1) {
       const float4_t v = *(const float4_t*)(part + i * stride + c * 4);
-      const float w = __builtin_amdgcn_exp2f(part[i * stride + hd] - off);
+      const float m = part[i * stride + hd] - off, w = __builtin_amdgcn_exp2f(m);
+      const float f = eight ? __builtin_amdgcn_exp2f(m + part[i * stride + hd + 2] - unit) : w;
       total += w * part[i * stride + hd + 1];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) o[k] += w * v[k];
+      for (int k = 0; k < 4; ++k) o[k] += f * v[k];
     }
   }
   if constexpr (MANY) {
@@ -69,8 +83,10 @@ __global__ __launch_bounds__(PC_THREADS) void paged_combine_kernel(PagedAttentio
   const float inv = total > 0.f || total != total ? 1.f / total : 0.f;
   uint16_t w[4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
-    w[k] = a.bf16 ? __builtin_bit_cast(uint16_t, (bf16_t)(o[k] * inv)) : __builtin_bit_cast(uint16_t, (half_t)(o[k] * inv));
+  for (int k = 0; k < 4; ++k) {
+    const float x = eight ? pa_times_power(o[k] * inv, unit) : o[k] * inv;
+    w[k] = a.bf16 ? __builtin_bit_cast(uint16_t, (bf16_t)x) : __builtin_bit_cast(uint16_t, (half_t)x);
+  }
   const int d = head * hd + c * 4;
   const int64_t at = a.out_mb > 0 ? packed_act_offset(r, d, a.out_mb) : (int64_t)r * a.ldo + d;
   *(pg_u2*)((uint16_t*)a.out + at) = pg_u2{(uint32_t)w[0] | (uint32_t)w[1] << 16, (uint32_t)w[2] | (uint32_t)w[3] << 16};

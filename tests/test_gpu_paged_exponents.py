@@ -151,3 +151,78 @@ def test_a_key_that_overflowed(dtype, form, new, sign, where):
     """It is held as the largest that codes can stand for.  Queries that are small and positive in its place look at nothing
     else, negative ones not at it; rows in front of it do not see it."""
     _with_infinities(dtype, form, new, 60, sign, 60 + new - 1 if where == "last" else 33, True, False)
+
+
+@pytest.mark.parametrize("where", ["last", "first"])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("key", [False, True], ids=["seen", "weighed"])
+@pytest.mark.parametrize("new", [1, 5])
+@pytest.mark.parametrize("dtype,form", FORMS, ids=IDS)
+def test_a_value_that_overflowed(dtype, form, new, key, sign, where):
+    """With an ordinary key, and with one that gives it all the weight or none: where it has none, or is not seen, it takes
+    nothing from the others."""
+    _with_infinities(dtype, form, new, 60, sign, 60 + new - 1 if where == "last" else 33, key, True)
+
+
+FEW = [(2, 64, 16, [1, 3], 90, 0, 0), (2, 64, 32, [20, 7], 31, 0, 0), (2, 80, 32, [5], 64, 0, 0), (4, 96, 64, [16], 130, 0, 0),
+       (4, 128, 16, [10, 1], 200, 40, 5), (2, 192, 32, [3], 3, 0, 0), (2, 256, 64, [9], 50, 33, 0), (2, 128, 64, [1], 3000, 0, 0),
+       (16, 64, 128, [2], 2500, 1500, 10)]
+
+
+@pytest.mark.parametrize("case", FEW, ids=lambda c: "h%d-d%d-p%d-n%d-at%d-w%d" % (c[:3] + (c[3][0],) + c[4:6]))
+@pytest.mark.parametrize("spread", [5, 10, 60])
+@pytest.mark.parametrize("dtype,form", FORMS, ids=IDS)
+def test_exponents_of_any_size(dtype, form, spread, case):
+    """Exponents of neighbouring positions up to 2^120 apart: keys (with queries that bring the largest scores to a few units)
+    and values, over tiles, splits, windows and heads that share keys."""
+    heads, hd, page, new, p, window, sinks = case
+    if dtype == torch.float16 and spread > 10:
+        spread = 14       # (values and queries are within fp16's range)
+    blocks = [-(-(p + n) // page) for n in new]
+    host = _pages(form, sum(blocks), 1, page, hd, 6)
+    g = torch.Generator().manual_seed(7)
+    host[2] = torch.randint(-spread, spread + 1, host[2].shape, generator=g).to(torch.int8)
+    host[3] = torch.randint(-spread, spread + 1, host[3].shape, generator=g).to(torch.int8) - 9
+    if spread == 10:      # far apart in one place only
+        host[2].clamp_(-5, 5)
+        host[3].clamp_(-14, -4)
+        host[3][:, 0, 11] = -30
+    table = _table(len(new), blocks, sum(blocks), 8)
+    cache = _cache(host)
+    top = float(host[2].max())
+    q = (torch.randn(sum(new), heads, hd, generator=g) * 2.0 ** (-top - 4)).to(dtype)
+    out = cache.attend(cache.batch(new, [p] * len(new), table.to(DEV)), q.to(DEV), window=window, sinks=sinks).cpu()
+    row = 0
+    for s, n in enumerate(new):
+        _check(host, table[s], q[row:row + n], p, out[row:row + n], window, sinks)
+        row += n
+
+
+@pytest.mark.parametrize("wide", [False, True], ids=["near", "far"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("new", [5])
+def test_a_nan_code_reaches_the_rows_that_see_it(dtype, new, wide):
+    """e4m3's NaN among values at a position that some rows of a tile see and others do not; then among keys."""
+    p, page = 60, 16
+    host = _pages(E4M3, 16, 1, page, 64, 17)
+    if wide:
+        host[3][:, 0, ::5] = -90
+    table = _table(1, [14], 16, 18)
+    q = torch.randn(new, 2, 64, generator=torch.Generator().manual_seed(19)).to(dtype)
+    place = lambda j: (int(table[0, j // page]), 0, j % page)  # noqa: E731
+    for j, d, code in ((p + 1, 5, 0x7f), (p + 4, 9, 0xff)):
+        a, h, o = place(j)
+        host[1].view(torch.uint8)[a, h, d, o] = code
+    out = _attend(_cache(host), table, q, p).float()
+    for i in range(new):
+        assert bool(torch.isnan(out[i, :, 5]).all()) == (i >= 1), i
+        assert bool(torch.isnan(out[i, :, 9]).all()) == (i >= 4), i
+        rest = [d for d in range(64) if d not in (5, 9)]
+        assert bool(torch.isfinite(out[i][:, rest]).all()), i
+    host = _pages(E4M3, 16, 1, page, 64, 17)
+    if wide:
+        host[2][:, 0, ::5] = -90
+    a, h, o = place(p + 3)
+    host[0].view(torch.uint8)[a, h, o, 7] = 0x7f
+    out = _attend(_cache(host), table, q, p)
+    assert bool(torch.isnan(out[3:]).all()) and bool(torch.isfinite(out[:3]).all())
