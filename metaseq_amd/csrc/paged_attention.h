@@ -573,7 +573,8 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
 // of a step of the product with V belong to eight consecutive keys: one 128-bit read of the transposed values.
 // 16-bit pages go to LDS directly (global_load_lds_dwordx4: 16 bytes a lane to consecutive places, from anywhere), 8-bit
 // ones through registers, where they become fp16: keys times 2^(e - the tile's largest e), values times 2^(e - E), E the largest so
-// far.  Chunks of 16 bytes of a row are exchanged by the row's number, so that reads of many rows meet all banks.
+// far, both exact while what is seen lies within 2^PT_NEAR of the largest; from the first tile on where it does not, codes stay
+// as they are and exponents go into scores and probabilities, as above (PT_NEAR).  Chunks of 16 bytes of a row are exchanged by the row's number, so that reads of many rows meet all banks.
 //
 // Bound by the vector units beside the matrix cores: a wave's tile of 128 dimensions is 32 products of 32 cycles and, for
 // 32 scores a lane, as many exponentials (16 cycles each) and some 150 other instructions, and the two waves that a SIMD
@@ -583,6 +584,11 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
 // 108 GFLOP, 180 us, 0.60 (tiles at the window's ends are computed whole).  Tried without gain: the scheduler's group
 // hints, wave priorities; without loads the kernel takes 0.9 of its time, without the product with V 0.87.
 constexpr int PT_BM = 128, PT_BN = 64, PT_THREADS = 256;
+// Exponents of keys of a tile, and of values so far, that rows of a workgroup see: up to so far apart one power of two for all
+// serves.  (A code is a multiple of 2^-9 and at most 448, so that fp16 holds it times 2^-12 exactly; a probability below
+// 2^-24 of the largest, which fp16 rounds to 2^-35, then is off by 2^-22 of what the largest adds.  us, four portions of 304 to
+// 513 tokens of 32 heads of 128 behind 1101 to 1536: near e4m3 118, int8 111, far apart from the first tile on 148 and 132.)
+constexpr int PT_NEAR = 12;
 
 typedef __attribute__((address_space(3))) void pt_lds_void;
 
@@ -664,7 +670,8 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
   const int tok = live ? rho / group : 0, g = live ? rho - tok * group : 0;
   const int pn = live ? position(rho) : -1;
   pg_u4 qf[KSTEPS];
-  float qs = a.scale * PA_LOG2E;
+  const float qs = a.scale * PA_LOG2E;
+  int eq = 0;  // 8 bits: the power of two that the row's queries stand for
   {
     const char* q = (const char*)a.q + (((int64_t)row0 + tok) * a.ldq + (int64_t)(h * group + g) * HD + hl * 8) * 2;
 #pragma unroll
@@ -687,7 +694,7 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
         for (int i = 0; i < 8; ++i) w[i] = (half_t)ldexpf((float)v[i], -k);
         qf[ks] = __builtin_bit_cast(pg_u4, w);
       }
-      qs = ldexpf(qs, k);
+      eq = k;
     }
   }
 
@@ -755,13 +762,14 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
   // 8 bits: chunks of 16 elements, registers in between.  Lane i of every wave has the exponents of key i; the factors that
   // follow from them reach the lanes that need them through LDS of the wave's own.
   constexpr int CB = HD / 16, KN = (PT_BN * CB + PT_THREADS - 1) / PT_THREADS, VN = (HD * 4 + PT_THREADS - 1) / PT_THREADS;
+  __shared__ __attribute__((aligned(16))) int8_t s_exponent[B8 ? 2 : 1][B8 ? 64 : 1];
   __shared__ __attribute__((aligned(16))) half_t s_factor[B8 ? PT_THREADS / 64 : 1][2][64];
   // Addresses that follow from the thread's number are formed anew for each tile where registers end: kept across the loop they
-  // would take others to scratch memory.  (us, kept and formed anew: 256 dimensions, int8 230 and 134, e4m3, which has the
-  // registers, 125 and 129; 128 dimensions 111 and 115)
+  // would take others to scratch memory.  (us: 256 dimensions in int8 230 with all of them kept, 155 with those of the keys'
+  // fragments, 141 with none; e4m3, which has the registers, 125 and 129; 128 dimensions 111 and 115)
   constexpr bool ANEW = F == PG_I8 && HD > 192;
   pg_u4 kr[B8 ? KN : 1], vr[B8 ? VN : 1];
-  int ke = 0, ve = 0;
+  int ke = 0, ve = 0, least = 127;  // of the lane's key; least: of values so far
   const int vg = threadIdx.x & 3;       // the sixteen keys that the thread's chunks of V belong to
   auto fetch = [&](int i, PtPages pg) {
     const int key0 = tiles.tile(i) * PT_BN, in = page - 1;
@@ -780,7 +788,8 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
     ve = a.v_exp[ul];
   };
   auto wave_most = [](int v) { return __builtin_amdgcn_readfirstlane((int)wave_max((float)v)); };
-  // (returns the exponents that the tile's keys and values are relative to)
+  // ek, ev: the exponents that the tile's keys and values are relative to.  Returns whether some are further from them than
+  // that allows (then the tile is no use).
   auto stage = [&](int i, int slot, PtPages pg, int& ek, int& ev) {
     const int key0 = tiles.tile(i) * PT_BN;
     int tid = threadIdx.x;
@@ -788,7 +797,9 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
     const bool mine = pg.of(lane >> 4) >= 0 && anyone(key0 + lane);
     ek = wave_most(mine ? ke : -127);
     ev = max(ev, wave_most(mine ? ve : -127));
-    // 2^(e - largest), 0 below what fp16 can be
+    least = min(least, mine ? ve : 127);
+    const uint64_t beyond = __ballot((mine && ke < ek - PT_NEAR) || least < ev - PT_NEAR);
+    // 2^(e - largest); 0 below what fp16 can be (keys that nobody sees)
     auto factor = [](int e) { return e < -24 ? (half_t)0.f : (half_t)__builtin_bit_cast(float, (uint32_t)(127 + min(e, 0)) << 23); };
     s_factor[wave][0][lane] = factor(ke - ek);
     s_factor[wave][1][lane] = factor(ve - ev);
@@ -820,6 +831,7 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
           *(half8_t*)(vt + row * 128 + pt_place<8>(2 * vg + e, row) * 16) = __builtin_bit_cast(half8_t, pa_operand<F>(w, e)) * f[e];
       }
     }
+    return beyond != 0;
   };
 
   // ---- fragments: K block ib, step ks: row with bits 2 and 3 of n32 exchanged, chunk 2 ks + hl.  V^T block db, step c (16
@@ -836,13 +848,14 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
   for (int d = 0; d < DBLK; ++d) o[d] = zero16;
   float m = -INFINITY, l = 0.f;
   int E = -127, ek = 0, ev = -127;  // what the accumulators are relative to, and this tile's keys and values
+  bool far = false;
   PtPages pg = {-1, -1, -1, -1}, next = pg;  // this tile's, and entries of the next one's
   if (it0 < it_end) {
     pg = checked(entries(it0), it0);
     next = entries(it0 + 1);
     if (B8) {
       fetch(it0, pg);
-      stage(it0, 0, pg, ek, ev);
+      far = stage(it0, 0, pg, ek, ev);
     } else {
       issue(it0, 0, pg);
     }
@@ -851,7 +864,8 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
   // loop, and with them for the tile just requested)
 #pragma unroll
   for (int ks = 0; ks < KSTEPS; ++ks) asm volatile("" : "+v"(qf[ks]));
-  for (int i = it0; i < it_end; ++i) {
+  int i = it0;
+  for (; i < it_end && !far; ++i) {
     const int slot = (i - it0) & 1;
     const int here = (pg.a >= 0 ? 1 : 0) | (pg.b >= 0 ? 2 : 0) | (pg.c >= 0 ? 4 : 0) | (pg.d >= 0 ? 8 : 0);
     if (!B8) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -892,16 +906,18 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
     const bool none = key0 > p_hi || w0 >= rows || (a.window > 0 && key0 + PT_BN - 1 <= p_lo - a.window && key0 >= a.sinks);
     // (zeros have the least exponent there is, queries of zeros too: below what fp32 can be any score is zero, but those of keys
     // that are not seen are -infinity, which a factor of zero would make NaN; above it a product of zero stays one)
-    const float to_score = B8 ? fminf(fmaxf(ldexpf(qs, ek), FLT_MIN), FLT_MAX) : qs;
+    const float to_score = B8 ? fminf(fmaxf(ldexpf(qs, ek + eq), FLT_MIN), FLT_MAX) : qs;
     // Two copies: tiles that every row of the wave sees whole, and others.
     auto attend = [&](auto edge) {
       constexpr bool EDGE = decltype(edge)::value;
       // (the order below is kept: left alone, the compiler requests a fragment right before its product and waits for it)
       float16_t sc[2];
       pg_u4 kf[AHEAD][2], vf[VAHEAD];
+      int krow_here = krow, half = hl;
+      if (ANEW) asm volatile("" : "+v"(krow_here), "+v"(half));
       auto k_at = [&](int ks, int ib) {
-        const int row = ib * 32 + krow;
-        return *(const pg_u4*)(kt + row * ROWB + pt_place<CH>(2 * ks + hl, row) * 16);
+        const int row = ib * 32 + krow_here;
+        return *(const pg_u4*)(kt + row * ROWB + pt_place<CH>(2 * ks + half, row) * 16);
       };
 #pragma unroll
       for (int ks = 0; ks < AHEAD; ++ks) kf[ks][0] = k_at(ks, 0), kf[ks][1] = k_at(ks, 1);
@@ -1016,8 +1032,149 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
     };
     if (whole) attend(std::false_type{});
     else if (!none) attend(std::true_type{});
-    if (B8 && i + 1 < it_end) stage(i + 1, slot ^ 1, pg, ek, ev);
+    if (B8 && i + 1 < it_end) far = stage(i + 1, slot ^ 1, pg, ek, ev);
     next = entries(i + 2);
+  }
+
+  // ---- 8 bits, exponents far apart: codes in LDS, every key's exponent in its score, every value's in its probability, relative
+  // to the row's own running maximum R as in the kernel above; one tile at a time ----
+  float power = B8 ? (float)E : 0.f;  // the accumulators are in units of 2^power
+  if constexpr (B8) {
+    float R = m == -INFINITY ? -INFINITY : (float)E;
+    // (what follows from the thread's number is formed here, not in front of the loop above, which needs the registers)
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int n32 = tid & 31, hl = (tid >> 5) & 1, krow = (n32 & ~12) | ((n32 & 4) << 1) | ((n32 & 8) >> 1);
+    for (; i < it_end; ++i) {
+      const int key0 = tiles.tile(i) * PT_BN;
+      const int here = (pg.a >= 0 ? 1 : 0) | (pg.b >= 0 ? 2 : 0) | (pg.c >= 0 ? 4 : 0) | (pg.d >= 0 ? 8 : 0);
+      fetch(i, pg);
+      __syncthreads();  // the tile before has been read
+      bool odd = false;
+#pragma unroll
+      for (int j = 0; j < KN; ++j) {
+        const int at = tid + j * PT_THREADS, row = at / CB, c = at % CB;
+        if ((PT_BN * CB) % PT_THREADS == 0 || at < PT_BN * CB) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) *(pg_u4*)(lds + row * ROWB + pt_place<CH>(2 * c + e, row) * 16) = pa_operand<F>(kr[j], e);
+        }
+      }
+      char* vt = lds + 2 * TILEB;
+      const uint32_t seen = pg.of(vg) >= 0 ? pa_seen<16>(key0 + vg * 16, g_lo, g_hi, a.window, a.sinks) : 0;
+#pragma unroll
+      for (int j = 0; j < VN; ++j) {
+        const int at = tid + j * PT_THREADS, row = at >> 2;
+        if ((HD * 4) % PT_THREADS == 0 || at < HD * 4) {
+          pg_u4 w = vr[j];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            w[k] = pa_keep<F>(w[k], seen >> (4 * k));
+            odd |= pa_not_finite<F>(w[k], 0) != 0;
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) *(pg_u4*)(vt + row * 128 + pt_place<8>(2 * vg + e, row) * 16) = pa_operand<F>(w, e);
+        }
+      }
+      if (wave == 0) s_exponent[0][tid] = (int8_t)ke, s_exponent[1][tid] = (int8_t)ve;
+      odd = __syncthreads_or(odd);  // the tile is complete
+      if (i + 1 < it_end) pg = checked(next, i + 1);
+      next = entries(i + 2);
+      if (key0 > p_hi || w0 >= rows) continue;
+      float z[32], c = qs, off;
+      {
+        float16_t sc[2];
+#pragma unroll
+        for (int ks = 0; ks < KSTEPS; ++ks)
+#pragma unroll
+          for (int ib = 0; ib < 2; ++ib) {
+            const int row = ib * 32 + krow;
+            sc[ib] = pt_mfma<F>(*(const pg_u4*)(lds + row * ROWB + pt_place<CH>(2 * ks + hl, row) * 16), qf[ks], ks == 0 ? zero16 : sc[ib]);
+          }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) z[j] = sc[j >> 4][j & 15];
+      }
+      auto exponent = [](pg_u2 w, int j) { return (int)(int8_t)(w[j >> 2] >> ((j & 3) * 8)); };
+      float top = -INFINITY;
+#pragma unroll
+      for (int g8 = 0; g8 < 4; ++g8) {
+        const pg_u2 x = *(const pg_u2*)&s_exponent[0][g8 * 16 + hl * 8];
+        const uint32_t sees = pa_seen<8>(key0 + g8 * 16 + hl * 8, pn, pn, a.window, a.sinks) * ((here >> g8) & 1);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float& s = z[g8 * 8 + j];
+          s = (sees >> j) & 1 ? ldexpf(s, exponent(x, j) + eq) : -INFINITY;
+          top = fmaxf(top, s);
+        }
+      }
+      top *= qs;
+      if (__ballot(top > m + PA_LAZY)) {
+        const float to = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, MSA_WAVE)));
+        l *= m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - to);
+        R -= m == -INFINITY ? 0.f : to - m;
+        m = to;
+      }
+      pa_relative(z, c, off, m, 0.f);
+      float sum = 0.f, most = -INFINITY;
+#pragma unroll
+      for (int g8 = 0; g8 < 4; ++g8) {
+        const pg_u2 x = *(const pg_u2*)&s_exponent[1][g8 * 16 + hl * 8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float& s = z[g8 * 8 + j];
+          s = __builtin_fmaf(s, c, -off);
+          sum += __builtin_amdgcn_exp2f(s + SHIFT);
+          s += (float)exponent(x, j);
+          most = fmaxf(most, s);
+        }
+      }
+      l += sum;
+      if (__ballot(most > R + PA_LAZY)) {
+        const float to = fmaxf(R, fmaxf(most, __shfl_xor(most, 32, MSA_WAVE)));
+        const float w = R == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(R - to);
+        R = to;
+#pragma unroll
+        for (int d = 0; d < DBLK; ++d)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) o[d][v] *= w;
+      }
+      if (F == PG_E4M3 && odd) {
+#pragma unroll 1
+        for (int j = 0; j < PT_BN; ++j) {
+          const bool mine = (pa_seen<1>(key0 + j, pn, pn, a.window, a.sinks) & (here >> (j >> 4))) != 0;
+          int hl4 = hl * 4;
+          asm volatile("" : "+v"(hl4));
+#pragma unroll
+          for (int db = 0; db < DBLK; ++db)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+              const int row = min(db * 32 + (v >> 2) * 8 + hl4 + (v & 3), HD - 1);
+              const uint16_t x = *(const uint16_t*)(vt + row * 128 + pt_place<8>(j >> 3, row) * 16 + (j & 7) * 2);
+              o[db][v] += mine && (x & 0x7fff) > 0x7c00 ? NAN : 0.f;
+            }
+        }
+      }
+      const float from = (R == -INFINITY ? 0.f : R) - SHIFT;
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        pg_u4 p;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const half2_t w = {(half_t)__builtin_amdgcn_exp2f(z[st * 8 + 2 * j] - from), (half_t)__builtin_amdgcn_exp2f(z[st * 8 + 2 * j + 1] - from)};
+          p[j] = __builtin_bit_cast(uint32_t, w);
+        }
+#pragma unroll
+        for (int db = 0; db < DBLK; ++db) {
+          const int row = min(db * 32 + n32, HD - 1);
+          pg_u4 v = *(const pg_u4*)(vt + row * 128 + pt_place<8>(2 * st + hl, row) * 16);
+          if (F == PG_E4M3 && odd) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = pa_finite<G>(v[k]);
+          }
+          o[db] = pt_mfma<F>(v, p, o[db]);
+        }
+      }
+    }
+    if (far) power = R == -INFINITY ? 0.f : R;
   }
 
   // ---- O^T: row n32, dimensions 32 db + 8 blk + 4 hl + r ----
@@ -1034,10 +1191,10 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
         const int d = db * 32 + blk * 8 + hl * 4;
         float4_t v;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = B8 ? ldexpf(o[db][blk * 4 + r], E) : o[db][blk * 4 + r];
+        for (int r = 0; r < 4; ++r) v[r] = o[db][blk * 4 + r];
         if (HD % 32 == 0 || d < HD) *(float4_t*)(to + d) = v;
       }
-    if (hl == 0) to[HD] = m, to[HD + 1] = l, to[HD + 2] = 0.f;
+    if (hl == 0) to[HD] = m, to[HD + 1] = l, to[HD + 2] = power;
     return;
   }
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
@@ -1049,7 +1206,7 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
       uint16_t w[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float z = (B8 ? ldexpf(o[db][blk * 4 + r], E) : o[db][blk * 4 + r]) * inv;
+        const float z = B8 ? pa_times_power(o[db][blk * 4 + r] * inv, power) : o[db][blk * 4 + r] * inv;
         w[r] = a.bf16 ? __builtin_bit_cast(uint16_t, (bf16_t)z) : __builtin_bit_cast(uint16_t, (half_t)z);
       }
       const int64_t at = a.out_mb > 0 ? packed_act_offset((int)row, head * HD + d, a.out_mb) : row * a.ldo + head * HD + d;

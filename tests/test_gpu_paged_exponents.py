@@ -145,10 +145,10 @@ def _with_infinities(dtype, form, new, p, sign, at, key, value):
 
 @pytest.mark.parametrize("where", ["last", "first"])
 @pytest.mark.parametrize("sign", [1.0, -1.0])
-@pytest.mark.parametrize("new", [1, 5])
+@pytest.mark.parametrize("new", [1, 5, 40, 150])
 @pytest.mark.parametrize("dtype,form", FORMS, ids=IDS)
 def test_a_key_that_overflowed(dtype, form, new, sign, where):
-    """It is held as the largest that codes can stand for.  Queries that are small and positive in its place look at nothing
+    """It is held as the largest that codes can stand for, in few rows and in portions.  Queries that are small and positive in its place look at nothing
     else, negative ones not at it; rows in front of it do not see it."""
     _with_infinities(dtype, form, new, 60, sign, 60 + new - 1 if where == "last" else 33, True, False)
 
@@ -156,7 +156,7 @@ def test_a_key_that_overflowed(dtype, form, new, sign, where):
 @pytest.mark.parametrize("where", ["last", "first"])
 @pytest.mark.parametrize("sign", [1.0, -1.0])
 @pytest.mark.parametrize("key", [False, True], ids=["seen", "weighed"])
-@pytest.mark.parametrize("new", [1, 5])
+@pytest.mark.parametrize("new", [1, 5, 40, 150])
 @pytest.mark.parametrize("dtype,form", FORMS, ids=IDS)
 def test_a_value_that_overflowed(dtype, form, new, key, sign, where):
     """With an ordinary key, and with one that gives it all the weight or none: where it has none, or is not seen, it takes
@@ -167,9 +167,12 @@ def test_a_value_that_overflowed(dtype, form, new, key, sign, where):
 FEW = [(2, 64, 16, [1, 3], 90, 0, 0), (2, 64, 32, [20, 7], 31, 0, 0), (2, 80, 32, [5], 64, 0, 0), (4, 96, 64, [16], 130, 0, 0),
        (4, 128, 16, [10, 1], 200, 40, 5), (2, 192, 32, [3], 3, 0, 0), (2, 256, 64, [9], 50, 33, 0), (2, 128, 64, [1], 3000, 0, 0),
        (16, 64, 128, [2], 2500, 1500, 10)]
+MANY = [(4, 64, 16, [150], 100, 0, 0), (2, 80, 32, [70], 31, 0, 0), (2, 96, 64, [129, 5], 64, 0, 0), (4, 128, 16, [100, 1], 200, 40, 5),
+        (2, 192, 32, [90], 3, 0, 0), (2, 256, 64, [64, 2], 50, 33, 0), (2, 128, 64, [140], 3000, 0, 0),
+        (2, 64, 128, [130], 2500, 1500, 10), (1, 128, 128, [300], 0, 0, 0)]
 
 
-@pytest.mark.parametrize("case", FEW, ids=lambda c: "h%d-d%d-p%d-n%d-at%d-w%d" % (c[:3] + (c[3][0],) + c[4:6]))
+@pytest.mark.parametrize("case", FEW + MANY, ids=lambda c: "h%d-d%d-p%d-n%d-at%d-w%d" % (c[:3] + (c[3][0],) + c[4:6]))
 @pytest.mark.parametrize("spread", [5, 10, 60])
 @pytest.mark.parametrize("dtype,form", FORMS, ids=IDS)
 def test_exponents_of_any_size(dtype, form, spread, case):
@@ -200,7 +203,7 @@ def test_exponents_of_any_size(dtype, form, spread, case):
 
 @pytest.mark.parametrize("wide", [False, True], ids=["near", "far"])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
-@pytest.mark.parametrize("new", [5])
+@pytest.mark.parametrize("new", [5, 40, 150])
 def test_a_nan_code_reaches_the_rows_that_see_it(dtype, new, wide):
     """e4m3's NaN among values at a position that some rows of a tile see and others do not; then among keys."""
     p, page = 60, 16
