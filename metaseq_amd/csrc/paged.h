@@ -27,11 +27,12 @@ struct PagedAttention {
   const int32_t *seq_start, *seq_pos, *table;
   int64_t ldq, ldo, table_stride;
   void* out;
-  // splits > 1: [M][heads][splits][hd + 4]: sums of p v in units of 2^unit, the maximum m that p is relative to (log2 units), the
+  // splits > 1: [rows][heads][splits][hd + 4]: sums of p v in units of 2^unit, the maximum m that p is relative to (log2 units), the
   // sum of p, unit (8 bits; 0 with 16), one more for the alignment
   float* partial;
   int M, nseq, heads, kv_heads, pages, page_log2, blocks, out_mb, window, sinks, splits, row_blocks, bf16, max_count;
   int few;      // sequences of at most so many (token, query head) rows of a key/value head are the wave kernel's
+  int part_tokens;  // rows of `partial`: so many for each sequence (0: those of the batch)
   int grouped;  // tile kernel: all workgroups of a (sequence, head) on one XCD
   float scale;
 };

@@ -548,7 +548,8 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
       const int rho = rho0 + rt * 16 + r, t = rho / group, head = h * group + rho - t * group;
       const int64_t row = (int64_t)row0 + t;
       if (a.splits > 1) {
-        float* part = a.partial + ((row * a.heads + head) * a.splits + split) * (HD + 4);
+        const int64_t at = a.part_tokens > 0 ? (int64_t)s * a.part_tokens + t : row;
+        float* part = a.partial + ((at * a.heads + head) * a.splits + split) * (HD + 4);
         *(float4_t*)(part + d) = o;
         if (d == 0) part[HD] = to, part[HD + 1] = total, part[HD + 2] = unit;
       } else {

@@ -14,7 +14,7 @@ namespace {
 // out = sum of the splits' sums, each relative to its own maximum.  hd / 4 threads have a (token, query head): a workgroup
 // takes several of them, or (MANY) one, for which groups of hd / 4 threads take every so manieth split and their sums are
 // added in the groups' order.  tokens: of the sequences of the wave kernel, at most so many each; 0: every row of those of
-// the tile kernel.  Bound by its reads, of few rows by latency: 32 splits of 32 heads of 128 of one token 4.7 us.  (us, attention
+// the tile kernel (with part_tokens > 0 that many, so that a workgroup's number is its row of the splits' sums).  Bound by its reads, of few rows by latency: 32 splits of 32 heads of 128 of one token 4.7 us.  (us, attention
 // and sum, one head to a workgroup and several: 1024 tokens of 32 heads of 128 in 2 splits 74 and 42, in 8 93 and 71, in 16 158
 // and 139; 4 tokens in 8 23.7 and 24.2, in 16 21.5 and 23.1, in 32 24 and 28)
 constexpr int PC_THREADS = 256, PC_MANY = 9;
@@ -33,7 +33,7 @@ __global__ __launch_bounds__(PC_THREADS) void paged_combine_kernel(PagedAttentio
   const int g = threadIdx.x / columns, c = threadIdx.x - g * columns;
   const int head = MANY ? blockIdx.y : blockIdx.y * groups + g;
   if (!MANY && (g >= groups || head >= a.heads)) return;
-  const float* part = a.partial + ((int64_t)r * a.heads + head) * splits * stride;
+  const float* part = a.partial + ((int64_t)(a.part_tokens > 0 ? (int)blockIdx.x : r) * a.heads + head) * splits * stride;
   float top = -INFINITY;
   if constexpr (MANY) {
     for (int i = lane; i < splits; i += 64) top = fmaxf(top, part[i * stride + hd]);
@@ -102,6 +102,7 @@ int few_of(const msa_paged_cache& c) { return c.format == MSA_PAGES_SAME ? 32 : 
 
 struct Plan {
   int row_tiles, row_blocks, splits;  // wave kernel (row_tiles 0: not launched)
+  int tokens;                         // of a sequence of its, at most
   int tile_blocks, tile_splits, grouped;  // tile kernel (tile_blocks 0: not launched)
 };
 
@@ -131,7 +132,7 @@ int tile_splits_of(int64_t groups, int64_t tiles, int hd) {
 }
 
 Plan plan_of(const msa_paged_cache& c, const msa_paged_batch& b, const msa_paged_attention_args& a) {
-  Plan p = {0, 0, 1, 0, 1, 0};
+  Plan p = {0, 0, 1, 1, 0, 1, 0};
   const int group = a.heads / c.kv_heads;
   const int64_t rows = (int64_t)b.max_count * group;
   // keys that a row block can see
@@ -147,6 +148,8 @@ Plan plan_of(const msa_paged_cache& c, const msa_paged_batch& b, const msa_paged
     const int kt = c.format == MSA_PAGES_SAME ? 32 : 64;
     const int64_t units = (int64_t)b.nseq * p.row_blocks * c.kv_heads;
     p.splits = splits_of(units, (keys_of(most) + kt - 1) / kt);
+    const int tokens = few / group;
+    p.tokens = tokens < 1 ? 1 : tokens < b.max_count ? tokens : b.max_count;
   }
   if (rows > few) {
     p.tile_blocks = (int)((rows + PT_BM - 1) / PT_BM);
@@ -162,10 +165,15 @@ Plan plan_of(const msa_paged_cache& c, const msa_paged_batch& b, const msa_paged
   return p;
 }
 
-// floats of one (row, head) in the workspace
-int64_t partial_floats(const Plan& p, int hd) {
-  const int64_t s = p.splits > p.tile_splits ? p.splits : p.tile_splits;
-  return s > 1 ? s * (hd + 4) : 0;
+// Rows of the wave kernel's sums in the workspace: where a batch has more than its sequences of that kernel can have (portions
+// beside single tokens), so many for each sequence, else the batch's own.
+int part_tokens_of(const Plan& p, const msa_paged_batch& b) { return (int64_t)b.nseq * p.tokens < b.M ? p.tokens : 0; }
+
+// The kernels run one after the other and use the same memory.
+int64_t partial_floats(const Plan& p, const msa_paged_batch& b, int heads, int hd) {
+  const int64_t few = part_tokens_of(p, b) > 0 ? (int64_t)b.nseq * p.tokens : b.M;
+  const int64_t rows = p.splits > 1 ? few * p.splits : 0, tiles = p.tile_splits > 1 ? (int64_t)b.M * p.tile_splits : 0;
+  return (rows > tiles ? rows : tiles) * heads * (hd + 4);
 }
 
 int check(const msa_paged_cache* c, const msa_paged_batch* b, const msa_paged_attention_args* a) {
@@ -187,7 +195,7 @@ extern "C" int64_t msa_paged_attention_workspace_bytes(const msa_paged_cache* c,
   const int rc = check(c, b, a);
   if (rc) return rc;
   if (b->M == 0 || b->nseq == 0 || b->max_count == 0) return 0;
-  return (int64_t)b->M * a->heads * partial_floats(plan_of(*c, *b, *a), c->hd) * 4;
+  return partial_floats(plan_of(*c, *b, *a), *b, a->heads, c->hd) * 4;
 }
 
 extern "C" int msa_paged_attention(const msa_paged_cache* c, const msa_paged_batch* b, const msa_paged_attention_args* a,
@@ -219,7 +227,7 @@ extern "C" int msa_paged_attention(const msa_paged_cache* c, const msa_paged_bat
   PagedAttention k = {a->q, c->k_pages, c->v_pages, c->k_exp, c->v_exp, b->seq_start, b->seq_pos, b->table, a->ldq, a->ldo,
                       b->table_stride, a->out, (float*)a->workspace, b->M, b->nseq, a->heads, c->kv_heads, c->pages,
                       paged_log2(c->page), b->blocks, a->out_mb, window, a->sinks, 1, 1,
-                      c->dtype == MSA_BF16, b->max_count, few_of(*c), p.grouped, a->scale};
+                      c->dtype == MSA_BF16, b->max_count, few_of(*c), 0, p.grouped, a->scale};
   hipStream_t s = (hipStream_t)stream;
   const int format = paged_format(*c);
   auto combine = [&](int tokens) {
@@ -243,14 +251,14 @@ extern "C" int msa_paged_attention(const msa_paged_cache* c, const msa_paged_bat
   if (p.row_tiles > 0) {
     k.splits = p.splits;
     k.row_blocks = p.row_blocks;
+    k.part_tokens = part_tokens_of(p, *b);
     switch (format) {
       case PG_F16: msa_launch_paged_rows_f16(k, c->hd, p.row_tiles, s); break;
       case PG_BF16: msa_launch_paged_rows_bf16(k, c->hd, p.row_tiles, s); break;
       case PG_E4M3: msa_launch_paged_rows_e4m3(k, c->hd, p.row_tiles, s); break;
       default: msa_launch_paged_rows_i8(k, c->hd, p.row_tiles, s); break;
     }
-    const int few = k.few / (a->heads / c->kv_heads);
-    combine(few < 1 ? 1 : few < b->max_count ? few : b->max_count);
+    combine(p.tokens);
     MSA_CHECK_LAUNCH("msa_paged_attention (rows)");
   }
   return MSA_OK;

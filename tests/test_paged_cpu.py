@@ -136,3 +136,25 @@ def test_python_refuses_what_it_can_see():
         PagedCache(t(3, 16, 2, 64).transpose(1, 2), t(3, 2, 64, 16))
     with pytest.raises(RuntimeError, match="GPU"):
         PagedCache(t(3, 2, 16, 64), t(3, 2, 64, 16))
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd", [(32, 8, 128), (12, 12, 64), (8, 1, 256)])
+@pytest.mark.parametrize("form", [_capi.MSA_PAGES_SAME, _capi.MSA_PAGES_INT8], ids=["same", "i8"])
+@pytest.mark.parametrize("tokens", [300, 8191])
+def test_single_tokens_beside_a_portion_need_little_more_than_alone(form, heads, kv_heads, hd, tokens):
+    """The sums of split keys have room for the rows whose keys are split - of every sequence as many as the kernel of few rows
+    takes, for the host does not say which have fewer - not for every row of the batch."""
+    lib = _capi.load()
+    c = _cache(format=form, kv_heads=kv_heads, hd=hd, k_exp=ONE, v_exp=ONE)
+
+    def need(new):
+        b = _batch(M=sum(new), nseq=len(new), max_count=max(new), min_count=min(new), key_bound=131072, blocks=2048, table_stride=2048)
+        n = lib.msa_paged_attention_workspace_bytes(ctypes.byref(c), ctypes.byref(b), ctypes.byref(_args(heads=heads)))
+        assert n >= 0
+        return n
+
+    few = max(1, (32 if form == _capi.MSA_PAGES_SAME else 64) * kv_heads // heads)   # tokens that the kernel of few rows takes
+    assert need([1]) > 0
+    for singles in (1, 7):
+        got = need([tokens] + [1] * singles)
+        assert got <= max(need([tokens]), (1 + singles) * need([few])) and got <= 64 << 20
