@@ -235,9 +235,10 @@ class PagedSlots:
 
     A slot takes pages as it grows.  Copies share the full pages of what they copy (``refs`` counts the holders).
     With ``window``, attention is over the last ``window`` positions and the first ``sinks``, and a page that no
-    position to come can see is given back by the next ``extend``.  ``lens``: positions each slot holds (int32 on the
-    device, negative: empty); ``host_lens``: the same on the host, except that decode steps count every slot of
-    ``stale`` as having taken part, which only the device knows."""
+    position to come can see is given back by the next ``extend`` or when pages run out.  ``lens``: positions each slot
+    holds (int32 on the device, negative: empty); ``host_lens``: the same on the host, except that decode steps count every
+    slot of ``stale`` as having taken part, which only the device knows: a slot may hold pages ahead of its positions
+    until ``reclaim`` takes them."""
 
     has_pads = False
     ragged = True
@@ -270,10 +271,8 @@ class PagedSlots:
         if self.refs[at] == 0:
             self.free.append(at)
 
-    def reserve(self, wanted):
-        """Pages for the positions [pos, pos + n) of every (slot, pos, n); all of them or, with ValueError, none."""
-        if any(pos + n > self.capacity for _, pos, n in wanted):
-            raise ValueError("a slot would hold more than %d positions" % self.capacity)
+    def _missing(self, wanted):
+        """What the positions [pos, pos + n) of every (slot, pos, n) lack: (slot, block) of new pages, and of copies."""
         new = [(s, b) for s, pos, n in wanted for b in range(pos // self.page, -(-(pos + n) // self.page))
                if int(self.host_table[s, b]) < 0]
         # a page that others hold too is not written to: whose next position lies in one gets a copy, but for the last
@@ -283,6 +282,31 @@ class PagedSlots:
             if at >= 0 and left.setdefault(at, self.refs[at]) > 1:
                 left[at] -= 1
                 copies.append((s, pos // self.page))
+        return new, copies
+
+    def reclaim(self):
+        """Takes back the pages behind what each slot holds (waits for the device if decode steps have left that open), and
+        those that its window has passed."""
+        self.exact_lens(list(self.stale))
+        for slot, n in enumerate(self.host_lens):
+            for b in range(-(-max(n, 0) // self.page), self.host_table.shape[1]):
+                if int(self.host_table[slot, b]) >= 0:
+                    self._drop(int(self.host_table[slot, b]))
+                    self.host_table[slot, b] = -1
+            if n >= 0:
+                self.holds(slot, n)
+
+    def reserve(self, wanted, again=None):
+        """Pages for the positions [pos, pos + n) of every (slot, pos, n); all of them or, with ValueError, none.  Where they are
+        short, after a ``reclaim``, which makes the slots' lengths exact: then for what ``again()`` returns.  Returns what
+        pages were reserved for."""
+        if any(pos + n > self.capacity for _, pos, n in wanted):
+            raise ValueError("a slot would hold more than %d positions" % self.capacity)
+        new, copies = self._missing(wanted)
+        if len(new) + len(copies) > len(self.free):
+            self.reclaim()
+            wanted = wanted if again is None else again()
+            new, copies = self._missing(wanted)
         if len(new) + len(copies) > len(self.free):
             raise ValueError("%d pages are needed, %d are free" % (len(new) + len(copies), len(self.free)))
         for s, b in new:
@@ -294,6 +318,7 @@ class PagedSlots:
             self._drop(old)
         if new or copies:
             self._upload()
+        return wanted
 
     def _copy_page(self, src, dst):
         for layer in self.layers:
@@ -320,7 +345,8 @@ class PagedSlots:
         self.stale.discard(slot)
         if self.window:
             first = max(-(-self.sinks // self.page), self._passed[slot])
-            past = max(first, (n - self.window + 1) // self.page)   # blocks below hold positions <= n - window only
+            # blocks below hold positions <= n - window only (a slot that steps took past its capacity has no more blocks)
+            past = max(first, min((n - self.window + 1) // self.page, self.host_table.shape[1]))
             for b in range(first, past):
                 if int(self.host_table[slot, b]) >= 0:
                     self._drop(int(self.host_table[slot, b]))

@@ -1122,11 +1122,14 @@ class TransformerDecoder(IncrementalDecoder):
         """One token for every slot of a paged cache (pads and empty slots sit the step out)."""
         B = cache.batch
         # (a slot that pads have kept below what the host counts already has its next position's page)
-        active = [(s, n) for s, n in enumerate(cache.host_lens) if 0 <= n < cache.capacity]
-        cache.reserve([(s, n, 1) for s, n in active])
+        def growing(takes_part):
+            return [(s, n, 1) for s, n in enumerate(cache.host_lens) if 0 <= n < cache.capacity and takes_part[s]]
+
+        # (short of pages: only for the slots that this step's tokens make longer)
+        active = cache.reserve(growing([True] * B), lambda: growing((tokens.view(-1) != self.padding_idx).tolist()))
         fixed = cache.__dict__.get("_decode_rows")
         step_len = cache.__dict__.setdefault("step_len", torch.empty(B, dtype=torch.int32, device=cache.device))
-        bound = max((n + 1 for _, n in active), default=1)
+        bound = max((n + 1 for _, n, _ in active), default=1)
         if fixed is None or fixed[0] < bound or fixed[0] > 2 * bound + 512:
             bound = min(cache.capacity, bound + 256)    # (how keys are split follows from it)
             batch = cache.layers[0].batch([1] * B, step_len, cache.table, key_bound=bound)
@@ -1135,7 +1138,7 @@ class TransformerDecoder(IncrementalDecoder):
         feat, _ = self._rows_core(lib, stream, tokens, B, 1, 1, 0, None, None, len_dev=cache.lens, step_len=step_len,
                                   paged=fixed[1], want_packed=B <= 64)
         check(lib.msa_advance_len(ptr(cache.lens), ptr(step_len), B, 1, stream))
-        for s, n in active:
+        for s, n, _ in active:
             cache.host_lens[s] = n + 1
             cache.stale.add(s)
         return feat

@@ -1,0 +1,63 @@
+"""Decode steps of OPT decoders over pools that are smaller than their slots' capacity.  Oracle and tolerances: those of the decoder's
+other tests over pages."""
+import pytest
+import torch
+
+from metaseq_amd import random_prompts
+from test_gpu_paged_decoder import _close, _model
+
+pytestmark = pytest.mark.gpu
+
+
+def _decode(d, cfg, cache, tokens):
+    """One step; ``tokens``: per slot the last token, or None for a pad.  Logits."""
+    last = torch.tensor([cfg.padding_idx if t is None else t for t in tokens], device="cuda")
+    logits = torch.zeros(len(tokens), cfg.vocab_size, dtype=torch.float16, device="cuda")
+    d.decode_slots(cache, last, tok_out=torch.zeros_like(last), score_out=torch.zeros(len(tokens), device="cuda"), logits_out=logits)
+    return logits
+
+
+@pytest.mark.parametrize("form", [torch.float16, torch.int8], ids=["f16", "i8"])
+def test_a_paused_slot_leaves_the_pool_to_the_others(form):
+    cfg, sd, model = _model()
+    d = model.decoder
+    cache = d.new_paged_cache(3, 96, pages=1 + 6 + 6, page=16, dtype=form)
+    ids = [random_prompts(cfg, 1, n, seed=n)[0].tolist() for n in (9, 20, 30)]
+    d.prefill_slots(cache, [0, 1, 2], [torch.tensor(t, device="cuda") for t in ids])
+    g = torch.Generator().manual_seed(1)
+    for step in range(60):     # (the prompts are 10, 21 and 31 tokens long)
+        toks = [None] + torch.randint(4, cfg.vocab_size, (2,), generator=g).tolist()
+        logits = _decode(d, cfg, cache, toks)
+        for s in (1, 2):
+            ids[s].append(toks[s])
+    for s in (1, 2):
+        _close(logits[s:s + 1], cfg, sd, torch.tensor(ids[s]), form, [len(ids[s]) - 1])
+    assert cache.lens.tolist() == [len(t) for t in ids]
+    # the one that was paused goes on where it was
+    ids[0].append(77)
+    logits = _decode(d, cfg, cache, [77, None, None])
+    _close(logits[:1], cfg, sd, torch.tensor(ids[0]), form, [len(ids[0]) - 1])
+    assert cache.lens.tolist() == [len(t) for t in ids]
+
+
+def test_decode_steps_in_a_window_go_on_in_a_small_pool():
+    cfg, sd, model = _model()
+    d = model.decoder
+    cache = d.new_paged_cache(2, 250, pages=2 * 5, page=16, window=40, sinks=5)
+    ids = [random_prompts(cfg, 1, n, seed=n)[0].tolist() for n in (30, 12)]
+    d.prefill_slots(cache, [0, 1], [torch.tensor(t, device="cuda") for t in ids])
+    g = torch.Generator().manual_seed(2)
+    for step in range(200):
+        toks = torch.randint(4, cfg.vocab_size, (2,), generator=g).tolist()
+        if step % 7 == 3:
+            toks[step % 2] = None
+        logits = _decode(d, cfg, cache, toks)
+        for s in (0, 1):
+            if toks[s] is not None:
+                ids[s].append(toks[s])
+                if step % 40 > 36:
+                    _close(logits[s:s + 1], cfg, sd, torch.tensor(ids[s]), torch.float16, [len(ids[s]) - 1], 40, 5)
+    assert cache.lens.tolist() == [len(t) for t in ids]
+    for s in (0, 1):
+        d.release_slot(cache, s)
+    assert sorted(cache.free) == list(range(10))
