@@ -1132,11 +1132,19 @@ class TransformerDecoder(IncrementalDecoder):
         bound = max((n + 1 for _, n, _ in active), default=1)
         if fixed is None or fixed[0] < bound or fixed[0] > 2 * bound + 512:
             bound = min(cache.capacity, bound + 256)    # (how keys are split follows from it)
-            batch = cache.layers[0].batch([1] * B, step_len, cache.table, key_bound=bound)
-            fixed = cache._decode_rows = (bound, PagedRows(lib, cache, batch, self.cfg.decoder_attention_heads,
-                                                           self.cfg.head_dim, cache.device))
-        feat, _ = self._rows_core(lib, stream, tokens, B, 1, 1, 0, None, None, len_dev=cache.lens, step_len=step_len,
-                                  paged=fixed[1], want_packed=B <= 64)
+            # int8 weights: chunks of at most 128 rows (_decode_chunks)
+            chunks = -(-B // self.PACKED_MAX_ROWS) if self.layers[0].fc2.qweight is not None else 1
+            size, parts = -(-B // chunks), []
+            for at in range(0, B, size):
+                part = slice(at, min(B, at + size))
+                batch = cache.layers[0].batch([1] * (part.stop - at), step_len[part], cache.table[part], key_bound=bound)
+                parts.append((part, PagedRows(lib, cache, batch, self.cfg.decoder_attention_heads, self.cfg.head_dim,
+                                              cache.device)))
+            fixed = cache._decode_rows = (bound, parts)
+        feats = [self._rows_core(lib, stream, tokens[part], part.stop - part.start, 1, 1, 0, None, None,
+                                 len_dev=cache.lens[part], step_len=step_len[part], paged=rows, want_packed=B <= 64)[0]
+                 for part, rows in fixed[1]]
+        feat = feats[0] if len(feats) == 1 else torch.cat(feats)
         check(lib.msa_advance_len(ptr(cache.lens), ptr(step_len), B, 1, stream))
         for s, n, _ in active:
             cache.host_lens[s] = n + 1

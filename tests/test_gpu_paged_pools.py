@@ -61,3 +61,32 @@ def test_decode_steps_in_a_window_go_on_in_a_small_pool():
     for s in (0, 1):
         d.release_slot(cache, s)
     assert sorted(cache.free) == list(range(10))
+
+
+@pytest.mark.parametrize("slots", [129, 200, 256])
+def test_int8_weights_take_many_slots_in_chunks(slots):
+    """No product of a step has more than 128 rows (the int8 product of more is many times slower); every slot has its result."""
+    cfg, _, model = _model(heads=2)
+    d = model.decoder
+    d.quantize_int8_()
+    cache = d.new_paged_cache(slots, 48, page=16)
+    ids = [random_prompts(cfg, 1, 3 + s % 20, seed=s)[0].tolist() for s in range(slots)]
+    for s in range(0, slots, 50):
+        d.prefill_slots(cache, list(range(s, min(s + 50, slots))), [torch.tensor(t, device="cuda") for t in ids[s:s + 50]])
+    sd = d.dequantized_state_dict()
+    sd = {k if k.startswith("decoder.") else "decoder." + k: v for k, v in sd.items()}
+    rows = []
+    linear = d._linear
+    d._linear = lambda lib, stream, x, lin, M, *a, **k: (rows.append(M), linear(lib, stream, x, lin, M, *a, **k))[1]
+    g = torch.Generator().manual_seed(3)
+    for step in range(3):
+        toks = torch.randint(4, cfg.vocab_size, (slots,), generator=g).tolist()
+        toks[step * 40 + 7] = None
+        logits = _decode(d, cfg, cache, toks)
+        for s, t in enumerate(toks):
+            ids[s] += [] if t is None else [t]
+        for s in (0, 63, 64, 99, 100, 127, 128, slots - 1):
+            if toks[s] is not None:
+                _close(logits[s:s + 1], cfg, sd, torch.tensor(ids[s]), torch.float16, [len(ids[s]) - 1])
+    assert rows and max(rows) <= 128
+    assert cache.lens.tolist() == [len(t) for t in ids]
