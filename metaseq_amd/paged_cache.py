@@ -363,9 +363,15 @@ class PagedSlots:
         self.stale.discard(slot)
 
     def copy_row(self, src, dst, n):
-        """Slot ``dst`` becomes slot ``src``, which holds ``n`` positions: it shares src's pages."""
+        """Slot ``dst`` becomes the first ``n`` positions of slot ``src``: it shares src's pages.  ValueError where src does not
+        hold so many, or has given back pages that dst's next position would see."""
         if src == dst:
             return
+        if n > self.host_lens[src]:   # (an upper bound of them; exact_lens would wait)
+            raise ValueError("slot %d holds no %d positions" % (src, n))
+        if any(int(self._blocks[src, b]) < 0 for b in range(-(-n // self.page)) if not self.window
+               or b * self.page < self.sinks or min((b + 1) * self.page, n) - 1 > n - self.window):
+            raise ValueError("slot %d has given back pages that a copy of %d positions would see" % (src, n))
         self.release_row(dst)
         for b in range(-(-n // self.page)):
             at = int(self._blocks[src, b])

@@ -88,6 +88,30 @@ def test_steps_past_the_capacity_leave_the_tables_alone():
     _sound(c)
 
 
+def test_copies_of_what_a_slot_does_not_hold_are_refused():
+    """More positions than it has; fewer, whose window reaches back to pages that are given back."""
+    c = _slots(3, 200, 30, window=40, sinks=5)
+    _grow(c, [(0, 0, 50)])
+    with pytest.raises(ValueError, match="holds no 51"):
+        c.copy_row(0, 1, 51)
+    with pytest.raises(ValueError, match="holds no 1"):
+        c.copy_row(2, 1, 1)
+    c.copy_row(0, 1, 20)
+    c.lens[1] = 20
+    for at in range(50, 150, 10):
+        _grow(c, [(0, at, 10)])
+    # 150: the next position sees 111 .. 149, blocks 1 .. 5 are gone; 135 would see 96, 134 95
+    assert [b for b in range(10) if int(c.host_table[0, b]) < 0] == [1, 2, 3, 4, 5]
+    for n in (134, 100, 60, 20):
+        with pytest.raises(ValueError, match="given back"):
+            c.copy_row(0, 2, n)
+    assert c.host_lens == [150, 20, -1]
+    for n in (150, 149, 135, 16, 3):
+        c.copy_row(0, 2, n)
+        assert c.host_lens[2] == n
+        _sound(c)
+
+
 @pytest.mark.parametrize("window", [0, 24])
 @pytest.mark.parametrize("seed", range(6))
 def test_any_order_of_calls(seed, window):
