@@ -378,7 +378,7 @@ class PagedSlots:
             if at >= 0:
                 self.refs[at] += 1
                 self._blocks[dst, b] = at
-        self.host_lens[dst], self._passed[dst] = n, self._passed[src]
+        self.host_lens[dst], self._passed[dst] = n, min(self._passed[src], -(-n // self.page))
         self._upload()
 
     def bytes(self):

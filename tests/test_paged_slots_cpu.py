@@ -112,6 +112,20 @@ def test_copies_of_what_a_slot_does_not_hold_are_refused():
         _sound(c)
 
 
+def test_a_short_copy_gives_back_its_own_pages():
+    """A copy of fewer positions than the source's window has passed: what it grows by comes back like any slot's."""
+    c = _slots(2, 200, 12, window=40, sinks=5)
+    for at in range(0, 150, 10):
+        _grow(c, [(0, at, 10)])
+    c.copy_row(0, 1, 16)
+    c.lens[1] = 16
+    c.release_row(0)
+    for at in range(16, 196, 10):
+        _grow(c, [(1, at, 10)])
+        _sound(c)
+        assert int((c.host_table[1] >= 0).sum()) <= 1 + 4, at
+
+
 @pytest.mark.parametrize("window", [0, 24])
 @pytest.mark.parametrize("seed", range(6))
 def test_any_order_of_calls(seed, window):
