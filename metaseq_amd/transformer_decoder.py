@@ -1034,7 +1034,9 @@ class TransformerDecoder(IncrementalDecoder):
         single tokens in any mix.  ``want``: per entry the offsets among its tokens whose logits are returned, fp16
         [sum of wanted, vocab] in that order (None: no logits; ``want_all``: every token's).  More than PORTION tokens
         run in portions."""
-        segments, ids = [], []
+        if not isinstance(cache, PagedSlots):
+            raise ValueError("not a paged cache")
+        segments, ids, entries = [], [], list(entries)
         cache.exact_lens([slot for slot, _ in entries])
         for slot, t in entries:
             if not 0 <= slot < cache.batch:
@@ -1048,6 +1050,10 @@ class TransformerDecoder(IncrementalDecoder):
             raise ValueError("a slot is named twice")
         if want_all:
             want = [range(n) for _, _, n in segments]
+        if want is not None:
+            want = [list(w) for w in want]
+            if len(want) != len(segments):
+                raise ValueError("%d entries, wanted places for %d" % (len(segments), len(want)))
         if want is not None and any(not 0 <= k < n for (_, _, n), w in zip(segments, want) for k in w):
             raise ValueError("a wanted place lies outside the entry's tokens")
         cache.reserve(segments)

@@ -90,3 +90,21 @@ def test_int8_weights_take_many_slots_in_chunks(slots):
                 _close(logits[s:s + 1], cfg, sd, torch.tensor(ids[s]), torch.float16, [len(ids[s]) - 1])
     assert rows and max(rows) <= 128
     assert cache.lens.tolist() == [len(t) for t in ids]
+
+
+def test_wanted_places_belong_to_entries():
+    """As many as entries; any iterables; nothing has run when they are refused."""
+    cfg, sd, model = _model()
+    d = model.decoder
+    cache = d.new_paged_cache(3, 40, page=16)
+    entries = [(0, [5, 6, 7]), (2, [8, 9])]
+    for want in ([[2]], [[2], [1], [0]], []):
+        with pytest.raises(ValueError, match="wanted places for"):
+            d.extend(cache, entries, want=want)
+    assert cache.host_lens == [-1] * 3 and len(cache.free) == 9
+    with pytest.raises(ValueError, match="not a paged cache"):
+        d.extend(d.new_slot_cache(2, 40), entries)
+    got = d.extend(cache, iter(entries), want=(iter(w) for w in ([2, 0], (1,))))
+    assert got.shape == (3, cfg.vocab_size)
+    _close(got[:2], cfg, sd, torch.tensor([5, 6, 7]), torch.float16, [2, 0])
+    _close(got[2:], cfg, sd, torch.tensor([8, 9]), torch.float16, [1])
