@@ -41,6 +41,11 @@ class PagedBatch:
         return self.c.key_bound
 
 
+def _no_gradients(*tensors):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError("metaseq_amd: the paged cache records no gradients; call it under torch.no_grad()")
+
+
 class PagedCache:
     """The pages of one layer.  The tensors are used as they are, not copied."""
 
@@ -168,7 +173,9 @@ class PagedCache:
 
     def append(self, batch, k, v):
         """Stores the keys and values ([rows, kv_heads, head_dim], fp16 or bf16, any row stride) of a batch's tokens at
-        their positions.  Nothing of this class records gradients."""
+        their positions.  Nothing of this class records gradients: what requires them is refused unless recording is off
+        (``torch.no_grad``)."""
+        _no_gradients(k, v)
         if k.dtype != v.dtype:
             raise ValueError("keys are %s, values %s" % (k.dtype, v.dtype))
         c = self._of(k.dtype, batch)
@@ -196,6 +203,7 @@ class PagedCache:
         output alike.  A token at position i sees positions j <= i; with ``window`` only those with j > i - window or
         j < ``sinks``.  ``scale``: default head_dim ** -0.5.  Rows of sequences that sit the call out keep what ``out``
         holds (or are undefined)."""
+        _no_gradients(q)
         if q.dim() != 3 or q.shape[1] % self.kv_heads or q.shape[1] == 0:
             raise ValueError("q must be [rows, heads, head_dim], heads a multiple of %d" % self.kv_heads)
         if not (0 <= window < 2 ** 31 and 0 <= sinks < 2 ** 31):

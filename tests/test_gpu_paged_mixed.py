@@ -23,3 +23,16 @@ def test_single_tokens_beside_a_portion(form, new, pos):
         out = cache.attend(batch, q.to(DEV), window=window, sinks=sinks).cpu()
         assert max(batch.workspaces.values()) > 0
         _check_attention(cache, _host(cache), new, pos, table, q, out, window, sinks)
+
+
+def test_what_requires_gradients_is_refused_while_they_are_recorded():
+    cache = _cache(_pages(torch.float16, 2, 2, 16, 64, 4))
+    batch = cache.batch([1], [0], torch.zeros(1, 1, dtype=torch.int32, device=DEV))
+    x = torch.randn(1, 2, 64, device=DEV).half()
+    with_grad = x.clone().requires_grad_()
+    for call in (lambda: cache.append(batch, with_grad, x), lambda: cache.append(batch, x, with_grad), lambda: cache.attend(batch, with_grad)):
+        with pytest.raises(RuntimeError, match="no gradients"):
+            call()
+        with torch.no_grad():
+            call()
+    assert torch.equal(cache.attend(batch, x), with_grad.detach())
