@@ -103,7 +103,8 @@ int few_of(const msa_paged_cache& c) { return c.format == MSA_PAGES_SAME ? 32 : 
 struct Plan {
   int row_tiles, row_blocks, splits;  // wave kernel (row_tiles 0: not launched)
   int tokens;                         // of a sequence of its, at most
-  int tile_blocks, tile_splits, grouped;  // tile kernel (tile_blocks 0: not launched)
+  int64_t tile_blocks;                // tile kernel (0: not launched)
+  int tile_splits, grouped;
 };
 
 // Splits of the keys, of at least PA_NW tiles each: up to 128 workgroups are made about 256 (one a CU); from there to 255, of
@@ -152,7 +153,7 @@ Plan plan_of(const msa_paged_cache& c, const msa_paged_batch& b, const msa_paged
     p.tokens = tokens < 1 ? 1 : tokens < b.max_count ? tokens : b.max_count;
   }
   if (rows > few) {
-    p.tile_blocks = (int)((rows + PT_BM - 1) / PT_BM);
+    p.tile_blocks = (rows + PT_BM - 1) / PT_BM;  // (of as many rows as the caller names: up to 2^40)
     const int64_t units = (int64_t)b.nseq * c.kv_heads;
     p.tile_splits = tile_splits_of(units * p.tile_blocks, (keys_of(PT_BM / group + 1) + PT_BN - 1) / PT_BN, c.hd);
     // A (sequence, head)'s blocks one after another on one XCD, whose L2 then has its keys, where all have about as many:
@@ -220,7 +221,7 @@ extern "C" int msa_paged_attention(const msa_paged_cache* c, const msa_paged_bat
   const Plan p = plan_of(*c, *b, *a);
   const int64_t units = (int64_t)b->nseq * c->kv_heads;
   MSA_REQUIRE((int64_t)b->nseq * few_of(*c) <= PG_MOST_GROUPS && units * p.row_blocks <= PG_MOST_GROUPS &&
-                  (units + 7) * p.tile_blocks * p.tile_splits <= PG_MOST_GROUPS,
+                  p.tile_blocks <= PG_MOST_GROUPS && (units + 7) * p.tile_blocks * p.tile_splits <= PG_MOST_GROUPS,
               MSA_ERR_INVALID_ARG, "msa_paged_attention: too many rows for one call");
   // (positions are below 2^30; a window that holds them all is none)
   const int window = a->window < (int64_t)b->blocks * c->page ? a->window : 0;
@@ -239,7 +240,7 @@ extern "C" int msa_paged_attention(const msa_paged_cache* c, const msa_paged_bat
   };
   if (p.tile_blocks > 0) {
     k.splits = p.tile_splits;
-    k.row_blocks = p.tile_blocks;
+    k.row_blocks = (int)p.tile_blocks;
     const bool ok = format == PG_F16    ? msa_launch_paged_tiles_f16(k, c->hd, s)
                     : format == PG_BF16 ? msa_launch_paged_tiles_bf16(k, c->hd, s)
                     : format == PG_E4M3 ? msa_launch_paged_tiles_e4m3(k, c->hd, s)

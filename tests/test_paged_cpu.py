@@ -158,3 +158,18 @@ def test_single_tokens_beside_a_portion_need_little_more_than_alone(form, heads,
     for singles in (1, 7):
         got = need([tokens] + [1] * singles)
         assert got <= max(need([tokens]), (1 + singles) * need([few])) and got <= 64 << 20
+
+
+@pytest.mark.parametrize("heads", [256, 4096, 32768, 65535])
+@pytest.mark.parametrize("max_count", [1 << 23, (1 << 24) - 1])
+@pytest.mark.parametrize("splits", [0, 1])
+def test_counts_whose_blocks_pass_32_bits_are_refused(heads, max_count, splits):
+    """A batch may name more rows for its longest sequence than it has; blocks for all of them must fit a launch."""
+    lib = _capi.load()
+    c = _cache(kv_heads=1)
+    b = _batch(M=200, nseq=1, max_count=max_count, min_count=0, key_bound=100000 * splits, blocks=2000, table_stride=2000)
+    a = _args(heads=heads, ldq=heads * 128, ldo=heads * 128)
+    assert lib.msa_paged_attention_workspace_bytes(ctypes.byref(c), ctypes.byref(b), ctypes.byref(a)) >= 0
+    if max_count * heads > 128 * ((1 << 24) - 1):
+        assert lib.msa_paged_attention(ctypes.byref(c), ctypes.byref(b), ctypes.byref(a), None) == -1
+        assert b"too many rows" in lib.msa_last_error()
