@@ -416,6 +416,8 @@ class ContinuousBatcher(_Front):
         import torch
 
         from . import _capi
+        from .paged_cache import PAGE_SIZES
+
         self._torch, self._capi = torch, _capi
         self.interface = interface
         self.model = interface.models[0]
@@ -429,8 +431,12 @@ class ContinuousBatcher(_Front):
         if cache_args is not None:
             if not hasattr(self.decoder, "new_paged_cache"):
                 raise ValueError("this decoder has no paged cache")
-            pages = cache_args.get("pages")
-            if pages is not None and pages < slots * -(-capacity // cache_args.get("page", 64)):
+            unknown = set(cache_args) - {"pages", "page", "dtype", "window", "sinks"}
+            pages, page = cache_args.get("pages"), cache_args.get("page", 64)
+            if unknown or page not in PAGE_SIZES:
+                raise ValueError("cache_args: " + ("no argument %s" % ", ".join(sorted(unknown)) if unknown else
+                                                   "pages of %s positions (of %s there are)" % (page, PAGE_SIZES)))
+            if pages is not None and pages < slots * -(-capacity // page):
                 raise ValueError("%d pages do not hold %d slots of %d positions" % (pages, slots, capacity))
         self.cache_args = cache_args
         self._stop: tuple = ()  # stop ids of the running batch

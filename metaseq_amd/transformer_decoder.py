@@ -22,7 +22,7 @@ from .checkpoint_utils import quantize_rows
 from .config import OPTConfig
 from .decoder_base import IncrementalDecoder, upload
 from .kv_cache import KVCache
-from .paged_cache import PagedRows, PagedSlots
+from .paged_cache import PAGE_SIZES, PagedRows, PagedSlots
 
 
 class _Affine(nn.Module):
@@ -1022,6 +1022,8 @@ class TransformerDecoder(IncrementalDecoder):
             raise ValueError("capacity %d outside 1..%d" % (capacity, self.max_positions()))
         if dtype == torch.bfloat16:
             raise ValueError("this decoder's keys and values are fp16")
+        if page not in PAGE_SIZES:
+            raise ValueError("pages of %s positions: pages of %s are supported" % (page, PAGE_SIZES))
         pages = slots * -(-capacity // page) if pages is None else int(pages)
         dev = device if device is not None else self.embed_tokens.weight.device
         cfg = self.cfg

@@ -108,3 +108,18 @@ def test_wanted_places_belong_to_entries():
     assert got.shape == (3, cfg.vocab_size)
     _close(got[:2], cfg, sd, torch.tensor([5, 6, 7]), torch.float16, [2, 0])
     _close(got[2:], cfg, sd, torch.tensor([8, 9]), torch.float16, [1])
+
+
+def test_bad_pages_are_refused_before_the_first_request():
+    from metaseq_amd import Dictionary, GeneratorInterface
+    from metaseq_amd.service import ContinuousBatcher
+
+    cfg, _, model = _model()
+    api = GeneratorInterface(model, Dictionary(cfg.vocab_size))
+    for page in (0, -16, 24, 512):
+        with pytest.raises(ValueError, match="positions"):
+            model.decoder.new_paged_cache(2, 100, page=page)
+        with pytest.raises(ValueError, match="positions"):
+            ContinuousBatcher(api, slots=4, capacity=64, cache_args=dict(page=page))
+    with pytest.raises(ValueError, match="no argument pgae"):
+        ContinuousBatcher(api, slots=4, capacity=64, cache_args=dict(pgae=16))
