@@ -107,14 +107,17 @@ struct Plan {
   int tile_splits, grouped;
 };
 
-// Splits of the keys, of at least PA_NW tiles each: up to 128 workgroups are made about 256 (one a CU); from there to 255, of
-// which some CUs would have two and others one, four each share better if they stay long; 256 and more are left alone.
-// (us, attention and sum in 1, 2, 4, 8 splits: 128 workgroups over 700 keys in fp16 15, 15, 15, 19, over 4000 68, 49, 50, 50, e4m3 39,
-// 29, 29, 32; 160 over 16000 264, 277, 204, 200; 192 272, 265, 233, 229, e4m3 134, 134, 129, 123, over 4112 45, 52, 51, 54; 256 e4m3
-// over 16000 158, 163, 160, 160; 1024 over 640 to 1281 98, 99, 101, 120; 8 over 131072 in int8 80 in 16, 56 in 32, 57 in 64, 60 in 128)
-int splits_of(int64_t groups, int64_t tiles) {
+// Splits of the keys, of at least PA_NW tiles each: up to 128 workgroups are made about 256 (one a CU).  Of 129 to 192 some CUs
+// would have two and others one: four each share better if they stay long (96 tiles), but for 8 bits of more than 64 dimensions, whose
+// workgroups overlap two to a CU.  More are left alone.  (us, attention and sum in 1, 2, 4 splits: 128 workgroups over 700 keys in fp16
+// 15, 15, 15, over 4000 68, 49, 50, e4m3 39, 29, 29; 8 over 131072 in int8 80 in 16, 56 in 32, 57 in 64, 60 in 128.  1 and 4 splits:
+// fp16, heads of 128, 160 over 2000, 3100, 6200, 16000 keys 40 and 39, 58 and 56, 111 and 103, 275 and 247; 192 42 and 42, 62 and
+// 61, 115 and 112, 287 and 273; 224 45 and 51, 67 and 74, 124 and 136, 309 and 332; of 256, 136 72 and 73, 108 and 105, 214 and 194,
+// 547 and 472; int8, heads of 64, 156 16 and 18, 24 and 21, 42 and 34, 98 and 74, 240 over 16000 101 and 102; e4m3, heads of 128, 136
+// over 6200 and 16000 56 and 56, 127 and 125, 192 59 and 64, 133 and 143, of 256, 136 101 and 109, 236 and 240)
+int splits_of(int64_t groups, int64_t tiles, bool overlap) {
   const int64_t most = (tiles + PA_NW - 1) / PA_NW;
-  int64_t s = groups <= 128 ? 256 / groups : groups < 256 && tiles >= 96 ? 4 : 1;
+  int64_t s = groups <= 128 ? 256 / groups : groups <= 192 && tiles >= 96 && !overlap ? 4 : 1;
   if (s > most) s = most;
   if (s > 128) s = 128;
   return s < 1 ? 1 : (int)s;
@@ -148,7 +151,7 @@ Plan plan_of(const msa_paged_cache& c, const msa_paged_batch& b, const msa_paged
     p.row_blocks = (int)((most + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
     const int kt = c.format == MSA_PAGES_SAME ? 32 : 64;
     const int64_t units = (int64_t)b.nseq * p.row_blocks * c.kv_heads;
-    p.splits = splits_of(units, (keys_of(most) + kt - 1) / kt);
+    p.splits = splits_of(units, (keys_of(most) + kt - 1) / kt, c.format != MSA_PAGES_SAME && c.hd > 64);
     const int tokens = few / group;
     p.tokens = tokens < 1 ? 1 : tokens < b.max_count ? tokens : b.max_count;
   }

@@ -36,3 +36,15 @@ def test_what_requires_gradients_is_refused_while_they_are_recorded():
         with torch.no_grad():
             call()
     assert torch.equal(cache.attend(batch, x), with_grad.detach())
+
+
+@pytest.mark.parametrize("new,pos", [([1] * 5, [3000, 0, 16, 700, 4000]), ([9, 1], [2000, 40]), ([200, 3], [1500, 10])], ids=str)
+@pytest.mark.parametrize("form", [torch.float16, E4M3, torch.int8], ids=["f16", "e4m3", "i8"])
+def test_a_call_repeats_itself_to_the_last_bit(form, new, pos):
+    blocks = [-(-(p + n) // 16) for n, p in zip(new, pos)]
+    cache = _cache(_pages(form, sum(blocks), 2, 16, 64, 5))
+    batch = cache.batch(new, pos, _table(len(new), blocks, sum(blocks), 6).to(DEV))
+    q = torch.randn(sum(new), 4, 64, generator=torch.Generator().manual_seed(7)).half().to(DEV)
+    first = cache.attend(batch, q)
+    for _ in range(3):
+        assert torch.equal(cache.attend(batch, q), first)
