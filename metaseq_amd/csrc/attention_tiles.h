@@ -1,8 +1,6 @@
 // What the attention kernels of hybrid decoders share.
 #pragma once
 
-#include <atomic>
-
 #include "common.h"
 
 namespace {
@@ -21,18 +19,6 @@ __device__ __forceinline__ bf16x8_t read_column8(const char* p, const char* p2) 
   const la_u2 hi = __builtin_bit_cast(la_u2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((la_lds_v4bf*)p2));
   const la_u4 w = {lo[0], lo[1], hi[0], hi[1]};
   return __builtin_bit_cast(bf16x8_t, w);
-}
-
-// allows a kernel that much dynamic LDS, once per device (`done`: one bit each)
-bool raise_lds(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return false;
-  const uint64_t bit = 1ull << dev;
-  if (done.load(std::memory_order_acquire) & bit) return true;
-  if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
-    return false;
-  done.fetch_or(bit, std::memory_order_release);
-  return true;
 }
 
 // keys of one split

@@ -5,6 +5,8 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <atomic>
+
 #include "../../include/metaseq_amd.h"
 #include "../../include/metaseq_hybrid.h"
 
@@ -284,4 +286,16 @@ __device__ __forceinline__ float block_max(float v, float* red) {
     t = fmaxf(t, i < nw ? r : t);
   }
   return t;
+}
+
+// allows a kernel that much dynamic LDS, once per device (`done`: one bit each)
+inline bool raise_lds(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return false;
+  const uint64_t bit = 1ull << dev;
+  if (done.load(std::memory_order_acquire) & bit) return true;
+  if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
+    return false;
+  done.fetch_or(bit, std::memory_order_release);
+  return true;
 }

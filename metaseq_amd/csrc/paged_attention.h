@@ -29,8 +29,6 @@
 #include <float.h>
 #include <math.h>
 
-#include <atomic>
-
 #include "paged.h"
 
 namespace {
@@ -48,17 +46,6 @@ struct PaFormat {
   static constexpr int NT = KT / 16;           // 16-key tiles of S^T in it
   static constexpr float SHIFT = F == PG_BF16 ? 0.f : 10.f;
 };
-
-// allows a kernel that much dynamic LDS, once per device (`done`: one bit each)
-bool pa_raise_lds(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return false;
-  const uint64_t bit = 1ull << dev;
-  if (done.load(std::memory_order_acquire) & bit) return true;
-  if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return false;
-  done.fetch_or(bit, std::memory_order_release);
-  return true;
-}
 
 __device__ __forceinline__ half8_t pa_e4m3(uint32_t lo, uint32_t hi) {
   const half2_t a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true);
@@ -1219,7 +1206,7 @@ template <int F, int HD>
 bool pa_launch_tiles(const PagedAttention& a, hipStream_t stream) {
   constexpr int bytes = 4 * PT_BN * HD * 2;
   static std::atomic<uint64_t> done{0};
-  if (!pa_raise_lds((const void*)paged_tile_kernel<F, HD>, bytes, done)) return false;
+  if (!raise_lds((const void*)paged_tile_kernel<F, HD>, bytes, done)) return false;
   const int64_t units = (int64_t)a.nseq * a.kv_heads, per = (int64_t)a.row_blocks * a.splits;
   const int64_t n = a.grouped ? (units + 7) / 8 * 8 * per : units * per;
   hipLaunchKernelGGL((paged_tile_kernel<F, HD>), dim3((unsigned)n), dim3(PT_THREADS), bytes, stream, a);
