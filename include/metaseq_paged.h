@@ -64,10 +64,12 @@ int msa_paged_read(const msa_paged_cache* c, const msa_paged_batch* b, void* k, 
  * head h uses key/value head h / (heads / kv_heads).  The row at position i sees positions j <= i, with window > 0 only
  * those of them with j > i - window or j < sinks:
  *   out = sum_j softmax_j(scale q . k_j) v_j
- * in fp32, rounded once; a row that sees nothing is zeros.  A row behind its table's positions sees what one at the last of
- * them would.  What stands at positions that no row of a sequence sees is never
- * used, whatever it is.  q [M, heads, hd] with row stride ldq; out with row stride ldo, or (out_mb > 0, MSA_F16, M <=
- * 128) in the packed activation layout of metaseq_amd.h with that many row blocks of heads * hd columns.
+ * with scores, maxima and sums in fp32; probabilities (relative to the maximum) are rounded to 16 bits for their products with
+ * values, the result once.  Over 8-bit pages neither a position that a row does not see nor a value that it gives no weight
+ * changes its result by more than such a rounding.  A row that sees nothing is zeros.  A row behind its table's positions
+ * sees what one at the last of them would.  What stands at positions that no row of a sequence sees is never used, whatever
+ * it is.  q [M, heads, hd] with row stride ldq; out with row stride ldo, or (out_mb > 0, MSA_F16, M <= 128) in the packed
+ * activation layout of metaseq_amd.h with that many row blocks of heads * hd columns.
  * workspace: at least msa_paged_attention_workspace_bytes of the same arguments (0: none needed), 16-byte aligned; calls
  * that may overlap need one each. */
 typedef struct {

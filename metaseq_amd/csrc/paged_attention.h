@@ -21,8 +21,8 @@
 // here, in pieces of 64 bytes a row or whole lines, in a kernel that does nothing else; whole lines past the caches at 6.7,
 // pieces of 64 bytes past them at 6.1, but an operand of the matrix cores is 64 bytes of sixteen rows.  Measured, heads of 128, all
 // keys and values: 64 sequences of 1280 keys, 32 heads, fp16, 1.34 GB, 221 us, 6.1 TB/s; 32 of 648 to 1282, 500 MB, 98 us, 5.1
-// (and 107 behind an append); 64 sequences, 72 heads, e4m3, 1.07 GB, 190 us, 5.6 TB/s; one of 131072 keys, 8 heads, int8,
-// 273 MB, 50 us, 5.4 TB/s, and 5 us for the sum of 32 splits; one of 58 keys, 12 heads of 64, 4.6 us.  Tried without gain: tiles
+// (and 107 behind an append); 64 sequences, 72 heads, e4m3, 1.07 GB, 191 us, 5.6 TB/s; one of 131072 keys, 8 heads, int8,
+// 273 MB, 52 us, 5.3 TB/s, and 5 us for the sum of 32 splits; one of 58 keys, 12 heads of 64, 4.7 us.  Tried without gain: tiles
 // of 64 keys of 16 bits (106 us instead of 108), one or two waves a unit, two to four workgroups a CU.
 #pragma once
 
@@ -562,20 +562,23 @@ __global__ __launch_bounds__(PA_NW * 64) void paged_rows_kernel(PagedAttention a
 // 16-bit pages go to LDS directly (global_load_lds_dwordx4: 16 bytes a lane to consecutive places, from anywhere), 8-bit
 // ones through registers, where they become fp16: keys times 2^(e - the tile's largest e), values times 2^(e - E), E the largest so
 // far, both exact while what is seen lies within 2^PT_NEAR of the largest; from the first tile on where it does not, codes stay
-// as they are and exponents go into scores and probabilities, as above (PT_NEAR).  Chunks of 16 bytes of a row are exchanged by the row's number, so that reads of many rows meet all banks.
+// as they are and exponents go into scores and probabilities, as above (PT_NEAR).  Chunks of 16 bytes of a row are exchanged
+// by the row's number, so that reads of many rows meet all banks.
 //
 // Bound by the vector units beside the matrix cores: a wave's tile of 128 dimensions is 32 products of 32 cycles and, for
 // 32 scores a lane, as many exponentials (16 cycles each) and some 150 other instructions, and the two waves that a SIMD
-// holds overlap little of it.  Measured, heads of 128, beside 1.14 PFLOP/s of a large product: 8192 tokens of 32 heads from
-// the start, fp16, 550 GFLOP, 0.64 to 0.72 ms, 0.76 to 0.86 PFLOP/s; four portions of 304 to 513 tokens of 32 heads behind
-// 1101 to 1536, 39.5 GFLOP, 79 us, 0.50; bf16, portions of 4096 and 2324 tokens of 32 heads on 8 with a window of 1024,
-// 108 GFLOP, 180 us, 0.60 (tiles at the window's ends are computed whole).  Tried without gain: the scheduler's group
+// holds overlap little of it; a short call by its longest workgroups too, all of which run at once.  Measured, heads of 128, a hundred
+// calls in a row (short runs, at a higher clock), beside 1.50 PFLOP/s of a large fp16 product and 1.58 of bf16: 8192 tokens of 32 heads
+// from the start, fp16, 550 GFLOP, 0.64 ms, 0.86 PFLOP/s; four portions of 304 to 513 tokens of 32 heads behind 1101 to 1536, 39.5
+// GFLOP, 92 us, 0.43 (78, 0.51), 480 workgroups of 26 tiles on the average and 33 at most; bf16, portions of 4096 and 2324 tokens of 32
+// heads on 8 with a window of 1024, 108 GFLOP, 198 us, 0.55 (181, 0.60; tiles at the window's ends are computed whole); the four portions in
+// e4m3 115, in int8 118.  Tried without gain: the scheduler's group
 // hints, wave priorities; without loads the kernel takes 0.9 of its time, without the product with V 0.87.
 constexpr int PT_BM = 128, PT_BN = 64, PT_THREADS = 256;
 // Exponents of keys of a tile, and of values so far, that rows of a workgroup see: up to so far apart one power of two for all
 // serves.  (A code is a multiple of 2^-9 and at most 448, so that fp16 holds it times 2^-12 exactly; a probability below
 // 2^-24 of the largest, which fp16 rounds to 2^-35, then is off by 2^-22 of what the largest adds.  us, four portions of 304 to
-// 513 tokens of 32 heads of 128 behind 1101 to 1536: near e4m3 118, int8 111, far apart from the first tile on 148 and 132.)
+// 513 tokens of 32 heads of 128 behind 1101 to 1536: near e4m3 115, int8 118, far apart from the first tile on 148 and 136.)
 constexpr int PT_NEAR = 12;
 
 typedef __attribute__((address_space(3))) void pt_lds_void;
@@ -958,7 +961,7 @@ __global__ __launch_bounds__(PT_THREADS, HD <= 128 ? 2 : 1) void paged_tile_kern
       float c = to_score, off;
       pa_relative(z, c, off, m, SHIFT);
       pg_u4 p[4];  // steps of sixteen keys of the product with V
-      float sum[2] = {0.f, 0.f};  // of the probabilities as they are rounded
+      float sum[2] = {0.f, 0.f};  // of the probabilities as they are rounded: weights that add up to one
       auto pair = [&](int st, int j) {
         const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(z[st * 8 + 2 * j], c, -off));
         const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(z[st * 8 + 2 * j + 1], c, -off));
