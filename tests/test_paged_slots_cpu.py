@@ -32,9 +32,8 @@ def _step(c, growing):
     """What a decode step does that ``growing`` slots take part in: the host counts all, the device those."""
     _reserve_a_step(c, growing)
     for s in growing:
-        at = int(c.lens[s]) // c.page
-        assert int(c.host_table[s, at]) >= 0 and c.refs[int(c.host_table[s, at])] == 1 and torch.equal(c.table, c.host_table) or \
-            int(c.table[s, at]) == int(c.host_table[s, at])
+        page = int(c.table[s, int(c.lens[s]) // c.page])
+        assert page >= 0 and c.refs[page] == 1 and page in c.host_table[s]
         c.lens[s] += 1
 
 
